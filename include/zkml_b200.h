@@ -394,6 +394,63 @@ int zkml_prove_aggregated_binding(zkml_ctx *ctx, const zkml_weight_claim *claims
  * cores.  c may be host memory or device memory of the context's GPU. */
 int zkml_matmul_m31(zkml_ctx *ctx, const uint32_t *a, size_t m, size_t k, const uint32_t *b, size_t n, uint32_t *c);
 
+/* ---- Forward operators with weights laid out once --------------------------------
+ * y = f(x W + b) + r and the gated block's h = f(x Wg + bg) * (x Wu + bu), mod p: what a
+ * Linear layer with its activation and residual, and a gated feed-forward block, compute
+ * before they are proved.  Exact for every M31 input.  A zkml_linear holds the weights in the
+ * layout the kernels read; it belongs to the context it was made with, is destroyed before
+ * it, and is not changed by calls, so calls on several streams (each with a workspace of its
+ * own) may use it at once. */
+typedef struct zkml_linear zkml_linear;
+
+/* Lay out W (k x n; element (i, j) at w[i * row_stride + j * col_stride], strides in words, so
+ * row-major and transposed weights both fit; host or device memory) and the bias (n words or
+ * NULL).  Runs on `stream` (NULL: the context's stream) and returns when the weights are in
+ * place; they are copied, the caller's memory is free again.  Refused while the stream is
+ * captured. */
+int zkml_linear_create(zkml_ctx *ctx, const uint32_t *w, size_t k, size_t n, size_t row_stride, size_t col_stride,
+                       const uint32_t *bias, void *stream, zkml_linear **out);
+/* Both projections of a gated block; the strides hold for both weights, each bias may be NULL. */
+int zkml_linear_create_gated(zkml_ctx *ctx, const uint32_t *w_gate, const uint32_t *w_up, size_t k, size_t n,
+                             size_t row_stride, size_t col_stride, const uint32_t *bias_gate,
+                             const uint32_t *bias_up, void *stream, zkml_linear **out);
+/* Waits for the work that uses the weights.  NULL is fine. */
+int zkml_linear_destroy(zkml_linear *lin);
+
+/* One call.  All pointers are memory of the context's GPU, strides are in words.  A row of x or
+ * residual may be anywhere (stride 0 repeats one row); outputs need a row stride of at least n
+ * and touch only their m x n words, and no output may overlap another argument, except that
+ * out may be the residual itself (same pointer and stride). */
+typedef struct {
+    const uint32_t *x; /* m x k activations */
+    size_t m, ldx;
+    int x_bits;     /* width the activations are quantised to: 8 ([-128, 127]), 16, or 31 (any element) */
+    int activation; /* f: 0 none, or a type tag (1 ReLU, 2 GELU, 3 Sigmoid, 4 Softmax-exp, 5 SiLU), applied
+                       to full M31 values as in zkml_prove_gkr_chain's forward pass; canonical result */
+    const uint32_t *residual; /* m x n added to f(x W + b), or NULL; not with gated weights */
+    size_t ld_residual;
+    uint32_t *out; /* y, or h for gated weights (m x n) */
+    size_t ld_out;
+    uint32_t *pre; /* optional: x W + b, for gated weights x Wg + bg (the activation's input, m x n) */
+    size_t ld_pre;
+    uint32_t *up; /* optional, gated weights only: x Wu + bu (m x n) */
+    size_t ld_up;
+    void *workspace; /* zkml_linear_workspace bytes, 256-byte aligned; free again once the call's work is done */
+    size_t workspace_bytes;
+    void *stream; /* cudaStream_t, NULL: the context's stream */
+} zkml_linear_call;
+
+/* Workspace of a call with m rows of x_bits activations. */
+int zkml_linear_workspace(const zkml_linear *lin, size_t m, int x_bits, size_t *out_bytes);
+/* Launches the call and returns; the outputs follow in stream order.  It neither allocates nor
+ * waits, so it can be captured into a CUDA graph.  An input word >= 2^31, or an activation
+ * outside x_bits, marks the handle: the outputs of that call are then unspecified words, and
+ * the next zkml_linear_check reports it. */
+int zkml_linear_forward(zkml_linear *lin, const zkml_linear_call *call);
+/* Waits for `stream` (NULL: the context's stream) and reports, once, whether a call since the
+ * last check met such a value. */
+int zkml_linear_check(zkml_linear *lin, void *stream);
+
 /* ---- Stepwise product sumcheck (multi-GPU building block) -------------------
  * The round loop of ZkmlOps::reduce_matmul_layer (backend.rs:141-178) one round
  * at a time, so that a caller can split one sumcheck across GPUs: rank g of G

@@ -157,6 +157,14 @@ _SIGS = {
     "zkml_selftest_wait_timeout": (C.c_int, [C.c_void_p, _u32]),
     "zkml_matmul_m31": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t,
                                   C.c_void_p]),
+    "zkml_linear_create": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t,
+                                     C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
+    "zkml_linear_create_gated": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t,
+                                           C.c_size_t, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
+    "zkml_linear_destroy": (C.c_int, [C.c_void_p]),
+    "zkml_linear_workspace": (C.c_int, [C.c_void_p, C.c_size_t, C.c_int, C.POINTER(C.c_size_t)]),
+    "zkml_linear_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "zkml_linear_check": (C.c_int, [C.c_void_p, C.c_void_p]),
     "zkml_shm_exchange_open": (C.c_int, [C.c_char_p, C.c_int, C.c_int, C.c_size_t, C.c_uint64, C.c_void_p]),
     "zkml_shm_exchange_close": (C.c_int, [C.c_void_p]),
     "zkml_prove_product_sharded": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_void_p,
@@ -1110,3 +1118,6 @@ def restrict_cols_noalloc(b, rows: int, cols: int, r_j, out, stream_ptr: Optiona
     n_rj = len(as_qm31_array(r_j))
     _check(lib().zkml_restrict_cols_noalloc(bb.ptr, rows, cols, r_ptr, n_rj, ob.ptr, ob.nbytes // 16,
                                             C.c_void_p(stream_ptr or 0)))
+
+
+from .forward import GatedLinearM31, LinearM31, gated_ffn_m31  # noqa: E402,F401

@@ -1,0 +1,260 @@
+"""Forward operators with weights laid out once (``zkml_linear_*`` of the C ABI).
+
+* ``LinearM31``      -- y = f(x W + b) + r mod p: a Linear layer with its activation and residual;
+* ``GatedLinearM31`` -- h = f(x Wg + bg) * (x Wu + bu) mod p: the up side of a gated feed-forward
+  block, both projections, the activation and the product in one launch;
+* ``gated_ffn_m31``  -- the two in a row: the whole gated feed-forward block.
+
+They compute what the layer reductions of this package prove: ``keep=True`` also returns the
+projections (the activation's input, and the second factor of the gated product).  Values are M31
+words; x is a CUDA tensor of int32 (or uint32) on the handle's device, used in place with any row
+stride, or a numpy uint32 array, which is copied and answered with numpy arrays.  Calls run on the
+device's current torch stream.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import numpy as np
+
+from . import ACTIVATION_TAGS, InvalidArgument, _check, _fast_fn, context, lib
+
+
+class _LinearCall(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("m", C.c_size_t), ("ldx", C.c_size_t), ("x_bits", C.c_int),
+                ("activation", C.c_int), ("residual", C.c_void_p), ("ld_residual", C.c_size_t),
+                ("out", C.c_void_p), ("ld_out", C.c_size_t), ("pre", C.c_void_p), ("ld_pre", C.c_size_t),
+                ("up", C.c_void_p), ("ld_up", C.c_size_t), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)]
+
+
+_TAGS = {None: 0, "none": 0, "relu": 1, **ACTIVATION_TAGS}
+_STREAM_LEGACY = 1  # cudaStreamLegacy: torch's default stream (0) by a handle that is not NULL
+
+
+def _tag(activation) -> int:
+    if isinstance(activation, str) or activation is None:
+        tag = _TAGS.get(activation.lower() if isinstance(activation, str) else None)
+        if tag is None:
+            raise InvalidArgument(1, f"unknown activation {activation!r}")
+        return tag
+    return int(activation)
+
+
+def _is_tensor(x) -> bool:
+    return hasattr(x, "data_ptr") and hasattr(x, "is_cuda")
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+class _Weights:
+    """Shared part of the two operators: the handle, the call and its checks."""
+
+    def __init__(self, weights, biases, device: Optional[int]):
+        first = weights[0]
+        if device is None:
+            device = first.device.index if _is_tensor(first) and first.is_cuda else 0
+        self.device = int(device)
+        self._handle = None
+        keep, ptrs, strides = [], [], []
+        for w in weights:
+            if len(w.shape) != 2:
+                raise InvalidArgument(1, "a weight is a matrix")
+            if tuple(w.shape) != tuple(first.shape):
+                raise InvalidArgument(1, "the weights of a gated block have the same shape")
+        if any(_strides(w) != _strides(first) for w in weights):
+            weights = [w.contiguous() if _is_tensor(w) else w for w in weights]
+        for w in weights:
+            w = self._words(w, "weight")
+            keep.append(w)
+            ptrs.append(_pointer(w))
+            strides.append(_strides(w))
+        if strides[0] != strides[-1]:
+            raise InvalidArgument(1, "the weights of a gated block are both tensors or both arrays")
+        self.k, self.n = int(first.shape[0]), int(first.shape[1])
+        for b in biases:
+            if b is None:
+                ptrs.append(None)
+                continue
+            if tuple(b.shape) != (self.n,):
+                raise InvalidArgument(1, f"a bias has {self.n} values")
+            b = self._words(b.contiguous() if _is_tensor(b) else np.ascontiguousarray(b), "bias")
+            keep.append(b)
+            ptrs.append(_pointer(b))
+        self._ctx = context(self.device)
+        h = C.c_void_p()
+        create = lib().zkml_linear_create_gated if len(weights) == 2 else lib().zkml_linear_create
+        rs, cs = strides[0]
+        _check(create(self._ctx.handle, *ptrs[:len(weights)], self.k, self.n, rs, cs, *ptrs[len(weights):],
+                      self._stream(), C.byref(h)))
+        self._handle = h
+
+    def close(self) -> None:
+        if self._handle:
+            lib().zkml_linear_destroy(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _stream(self) -> int:
+        torch = _torch()
+        if not torch.cuda.is_available():
+            return 0
+        return torch.cuda.current_stream(self.device).cuda_stream or _STREAM_LEGACY
+
+    def _words(self, x, name):
+        """x as words the library can read: a tensor of 32-bit integers (CUDA: on this device), or an array."""
+        if not _is_tensor(x):
+            x = np.asarray(x)
+            if x.dtype not in (np.uint32, np.int32):
+                raise InvalidArgument(1, f"{name}: M31 words are uint32 or int32")
+            return x if all(s >= 0 for s in x.strides) else np.ascontiguousarray(x)
+        torch = _torch()
+        if x.dtype not in (torch.int32, torch.uint32):
+            raise InvalidArgument(1, f"{name}: M31 words are int32 or uint32")
+        if x.is_cuda and x.device.index != self.device:
+            raise InvalidArgument(1, f"{name} is on {x.device}, the weights are on cuda:{self.device}")
+        return x
+
+    def _rows(self, x, width, name, m=None):
+        """(pointer, rows, row stride) of a matrix of words on this device; one row may be 1-D."""
+        x = self._words(x, name)
+        if not x.dim() or x.shape[-1] != width:
+            raise InvalidArgument(1, f"{name} has rows of {width} words")
+        if width > 1 and x.stride(-1) != 1:
+            raise InvalidArgument(1, f"{name}: the words of a row must be contiguous")
+        lead = [(int(d), int(st)) for d, st in zip(x.shape[:-1], x.stride()[:-1]) if d != 1]
+        rows, ld = 1, width
+        if lead:
+            ld = lead[-1][1]
+            for d, st in reversed(lead):
+                if st != ld * rows and d:
+                    raise InvalidArgument(1, f"{name}: the rows must be at one stride")
+                rows *= d
+        if not x.is_cuda:
+            raise InvalidArgument(1, f"{name} is not on cuda:{self.device}")
+        if m is not None and rows != m:
+            raise InvalidArgument(1, f"{name} has {rows} rows, x has {m}")
+        return x.data_ptr(), rows, ld
+
+    def _call(self, x, activation, residual, out, pre, up, keep, x_bits, check):
+        if self._handle is None:
+            raise InvalidArgument(1, "the weights were closed")
+        torch = _torch()
+        if check and torch.cuda.is_current_stream_capturing():
+            raise InvalidArgument(1, "the check waits for the stream; pass check=False while it is captured")
+        c = _LinearCall()
+        c.x, m, c.ldx = self._rows(x, self.k, "x")
+        c.m, c.x_bits, c.activation = m, int(x_bits), _tag(activation)
+        if residual is not None:
+            if residual.dim() == 1 and m != 1:
+                residual = residual.unsqueeze(0).expand(m, self.n)  # one row for every token
+            c.residual, _, c.ld_residual = self._rows(residual, self.n, "residual", m)
+        shape = tuple(x.shape[:-1]) + (self.n,)
+        dev = x.device
+        results = []
+        for name, t, want in (("out", out, True), ("pre", pre, keep), ("up", up, keep and self._gated)):
+            if t is None and want:
+                t = torch.empty(shape, dtype=torch.int32, device=dev)
+            if t is not None:
+                p, _, ld = self._rows(t, self.n, name, m)
+                setattr(c, name, p)
+                setattr(c, "ld_" + name, ld)
+                results.append(t)
+        need = C.c_size_t(0)
+        _check(lib().zkml_linear_workspace(self._handle, m, c.x_bits, C.byref(need)))
+        if need.value:
+            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+            c.workspace, c.workspace_bytes = ws.data_ptr(), need.value
+        c.stream = self._stream()
+        _check(_fast_fn("zkml_linear_forward", 2)(self._handle.value, C.addressof(c)))
+        if check:
+            self.check()
+        return results
+
+    def check(self) -> None:
+        """Waits for the current stream; raises if a call since the last check met a word >= 2^31 or an
+        activation that does not fit its x_bits."""
+        _check(lib().zkml_linear_check(self._handle, self._stream()))
+
+    def _run(self, x, activation, residual, out, pre, up, keep, x_bits, check):
+        if _is_tensor(x):
+            r = self._call(x, activation, residual, out, pre, up, keep, x_bits, check)
+            return r[0] if len(r) == 1 else tuple(r)
+        if out is not None or pre is not None or up is not None:
+            raise InvalidArgument(1, "output tensors go with a tensor x")
+        r = self._call(self._upload(x, "x"), activation, None if residual is None else self._upload(residual, "residual"),
+                       None, None, None, keep, x_bits, True)
+        r = [t.cpu().numpy().view(np.uint32) for t in r]
+        return r[0] if len(r) == 1 else tuple(r)
+
+    def _upload(self, x, name):
+        if _is_tensor(x):
+            return x
+        w = np.ascontiguousarray(self._words(x, name)).view(np.int32)
+        return _torch().from_numpy(w).to(f"cuda:{self.device}")
+
+
+def _strides(w):
+    if _is_tensor(w):
+        return tuple(int(s) for s in w.stride())
+    w = np.asarray(w)
+    return tuple(int(s) // w.itemsize for s in w.strides)
+
+
+def _pointer(w) -> int:
+    return w.data_ptr() if _is_tensor(w) else w.ctypes.data
+
+
+class LinearM31(_Weights):
+    """y = f(x W + b) + r mod p.  weight: k x n M31 words (a CUDA tensor, also transposed, or an
+    array), bias: n words or None; both are copied into the kernels' layout, once."""
+
+    _gated = False
+
+    def __init__(self, weight, bias=None, device: Optional[int] = None):
+        super().__init__([weight], [bias], device)
+
+    def __call__(self, x, activation=None, residual=None, out=None, pre=None, keep: bool = False, x_bits: int = 31,
+                 check: bool = True):
+        """x: (..., k); returns y (..., n), or (y, x W + b) with keep (or a tensor for pre).
+
+        activation: None, "relu", "gelu", "sigmoid", "softmax", "silu" or a type tag; residual: as y, or
+        one row of n words for all; out / pre: int32 tensors to write, of any row stride (out may be the
+        residual); x_bits: the width x is quantised to (8, 16, or 31 for any field element).
+        check=True waits for the call and raises InvalidArgument for a word >= 2^31 or an x outside
+        x_bits; check=False returns at once (and can be captured into a CUDA graph), and check() reports
+        later."""
+        return self._run(x, activation, residual, out, pre, None, keep, x_bits, check)
+
+
+class GatedLinearM31(_Weights):
+    """h = f(x Wg + bg) * (x Wu + bu) mod p; weights and biases as LinearM31's."""
+
+    _gated = True
+
+    def __init__(self, w_gate, w_up, bias_gate=None, bias_up=None, device: Optional[int] = None):
+        super().__init__([w_gate, w_up], [bias_gate, bias_up], device)
+
+    def __call__(self, x, activation="silu", out=None, gate=None, up=None, keep: bool = False, x_bits: int = 31,
+                 check: bool = True):
+        """x: (..., k); returns h (..., n), or (h, x Wg + bg, x Wu + bu) with keep; the rest as
+        LinearM31's call."""
+        return self._run(x, activation, None, out, gate, up, keep, x_bits, check)
+
+
+def gated_ffn_m31(x, gated: GatedLinearM31, down: LinearM31, activation="silu", residual=None, x_bits: int = 31,
+                  check: bool = True):
+    """A gated feed-forward block: (f(x Wg + bg) * (x Wu + bu)) Wd + bd + r mod p.  h is a full field
+    element, so the down projection takes it as one, whatever x_bits."""
+    h = gated(x, activation=activation, x_bits=x_bits, check=check)
+    return down(h, residual=residual, x_bits=31, check=check)
