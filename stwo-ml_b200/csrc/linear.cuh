@@ -1,4 +1,4 @@
-// Forward operators with weights laid out once: internal interface of linear_kernels.cu.
+// Forward operators with weights laid out once: interface of linear_kernels.cu.
 #pragma once
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -7,27 +7,62 @@
 namespace zk {
 
 // Bits of a handle's status word.
-constexpr uint32_t LIN_BAD_VALUE = 1u;   // an input word >= 2^31
-constexpr uint32_t LIN_BAD_RANGE = 2u;   // an activation that does not fit the declared width
+constexpr uint32_t LIN_BAD_VALUE = 1u;  // an input word >= 2^31
+constexpr uint32_t LIN_BAD_RANGE = 2u;  // an activation that does not fit the declared width
+constexpr uint32_t LIN_TIMEOUT = 4u;    // a bounded wait ran out
 
-// What one launch reads and writes.  Strides are in words; a row of x / residual may repeat
-// (stride 0).  n is the output width (per projection for gated weights).
-struct LinearArgs {
+// Tiles: 128 rows (outputs) x 128 bytes (K) of weights.
+constexpr uint32_t LIN_ROWS = 128;
+constexpr uint32_t LIN_KB = 128;
+constexpr uint32_t LIN_TILE_BYTES = LIN_ROWS * LIN_KB;
+
+// Weights in the kernels' layout: per plane, row tile and K tile 16 KiB, row r of a tile at
+// 128 r with its 16-byte chunk c at c ^ (r & 7) (the 128-byte swizzle).  Plane p holds the signed
+// byte digit of 256^p.  Row r of tile t is output 128 t + r, or for gated weights, in every 32
+// rows, 16 gate rows and then the 16 up rows of the same outputs (64 outputs a tile), so both
+// projections of an output meet in one warp's lanes l and l + 16.
+struct PackedWeights {
+    const uint8_t* tiles = nullptr;
+    const uint32_t* base = nullptr;  // 2 x row slots: bias, and bias + 128 (column sum of the weights), mod P
+    uint32_t k = 0, n = 0, k_tiles = 0, n_tiles = 0, planes = 0;
+    bool gated = false;
+};
+inline uint32_t lin_outputs_per_tile(bool gated) { return gated ? LIN_ROWS / 2 : LIN_ROWS; }
+
+// Packs w (and w2 for gated weights); columns' sums are added into sums (one u64 per row slot,
+// zeroed by the caller).  status[0] collects LIN_BAD_VALUE, status[1] the planes the values need.
+void launch_linear_pack(const uint32_t* w, const uint32_t* w2, size_t rs, size_t cs, const PackedWeights& p,
+                        uint8_t* tiles, unsigned long long* sums, uint32_t* status, cudaStream_t s);
+// base[] from the sums and the bias (NULL: zero).
+void launch_linear_base(const unsigned long long* sums, const uint32_t* bias, const uint32_t* bias2,
+                        const PackedWeights& p, uint32_t* base, uint32_t* status, cudaStream_t s);
+
+// One call.  Strides are in words.
+struct LinearIO {
     const uint32_t* x;
-    const uint32_t* w;        // k x n, row major (gated: k x 2n, gate then up in each row)
-    const uint32_t* bias;     // n words (gated: 2n) or NULL
     const uint32_t* residual;
     uint32_t *out, *pre, *up;
     uint32_t* status;
     size_t ldx, ld_res, ld_out, ld_pre, ld_up;
-    uint32_t m, k, n;
-    int x_bits, activation;
-    bool gated;
+    uint32_t m;
+    int activation;
 };
 
-void launch_linear_simple(const LinearArgs& a, cudaStream_t s);
-// dst[i][off + j] = src[i * rs + j * cs] mod P, row pitch ld; sets LIN_BAD_VALUE in *status.
-void launch_linear_lay_out(const uint32_t* src, uint32_t k, uint32_t n, size_t rs, size_t cs, uint32_t* dst,
-                           size_t ld, size_t off, uint32_t* status, cudaStream_t s);
+// How a call is split: fixed by the sizes alone.
+struct LinearPlan {
+    uint32_t digits;    // byte digits per activation: 1, 2 or 4
+    uint32_t tokens;    // tokens per tile
+    uint32_t m_tiles;
+    uint32_t tiles;     // m_tiles x n_tiles
+    uint32_t sk_tiles;  // the first tiles are cut at even shares of their units, the others are whole
+    uint32_t ctas;
+    uint32_t stages;
+    uint32_t slots;     // partial-sum slots per block
+    size_t digits_off, slots_off, bytes;  // workspace: counters, digit tiles, slots
+};
+LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms);
+cudaError_t linear_configure();  // per device, before the first launch
+cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, void* workspace,
+                          cudaStream_t s);
 
 }  // namespace zk

@@ -8,12 +8,11 @@
 
 struct zkml_linear {
     zkml_ctx* ctx = nullptr;
-    uint32_t k = 0, n = 0;
-    bool gated = false;
-    zk::DevBuf w, bias, status;
+    zk::PackedWeights w;
+    zk::DevBuf tiles, base, status;
     void release() {
-        w.release();
-        bias.release();
+        tiles.release();
+        base.release();
         status.release();
     }
 };
@@ -77,7 +76,7 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     if (k == 0 || n == 0) return set_error(ZKML_ERR_INVALID_ARG, "empty matrix");
     if (k > (1u << 30) || n > (1u << 30) || k * n > ((size_t)1 << 34))
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
-    if (rs > ((size_t)1 << 34) || cs > ((size_t)1 << 34))
+    if (rs > ((size_t)1 << 34) || cs > ((size_t)1 << 34) || (k - 1) * rs + (n - 1) * cs > ((size_t)1 << 36))
         return set_error(ZKML_ERR_INVALID_ARG, "weight stride too large");
     DeviceGuard guard;
     ZK_CUDA(cudaSetDevice(ctx->device));
@@ -86,37 +85,34 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     ZK_CUDA(cudaStreamIsCapturing(s, &cap));
     if (cap != cudaStreamCaptureStatusNone)
         return set_error(ZKML_ERR_INVALID_ARG, "weights cannot be laid out while the stream is captured");
-    const size_t span = ((k - 1) * rs + (n - 1) * cs + 1) * 4;
+    ZK_CUDA(linear_configure());
     zkml_linear* lin = new zkml_linear();
     struct Drop {
         zkml_linear*& l;
-        DevBuf stage;
-        ~Drop() {
-            stage.release();
+        DevBuf stage[4], sums;
+        ~Drop() {  // cudaFree waits for the kernels that use these
+            for (DevBuf& b : stage) b.release();
+            sums.release();
             if (l) {
                 l->release();
                 delete l;
             }
         }
-    } drop{lin, {}};
+    } drop{lin, {}, {}};
     lin->ctx = ctx;
-    lin->k = (uint32_t)k;
-    lin->n = (uint32_t)n;
-    lin->gated = parts == 2;
+    PackedWeights& w = lin->w;
+    w.k = (uint32_t)k;
+    w.n = (uint32_t)n;
+    w.gated = parts == 2;
+    w.k_tiles = (uint32_t)((k + LIN_KB - 1) / LIN_KB);
+    w.n_tiles = (uint32_t)((n + lin_outputs_per_tile(w.gated) - 1) / lin_outputs_per_tile(w.gated));
+    const size_t slots = (size_t)w.n_tiles * LIN_ROWS, plane = (size_t)w.n_tiles * w.k_tiles * LIN_TILE_BYTES;
+    const uint32_t* dev[4] = {};  // weights, then biases
     int rc;
-    if ((rc = lin->status.ensure(16)) || (rc = lin->w.ensure((size_t)parts * k * n * 4))) return rc;
-    const bool any_bias = biases[0] || (parts == 2 && biases[1]);
-    if (any_bias && (rc = lin->bias.ensure((size_t)parts * n * 4))) return rc;
-    ZK_CUDA(cudaMemsetAsync(lin->status.ptr, 0, 16, s));
     for (int g = 0; g < 2 * parts; g++) {
         const bool is_bias = g >= parts;
         const uint32_t* src = is_bias ? biases[g - parts] : ws[g];
-        if (is_bias && !any_bias) continue;
-        if (is_bias && !src) {
-            ZK_CUDA(cudaMemsetAsync(lin->bias.as<uint32_t>() + (size_t)(g - parts) * n, 0, n * 4, s));
-            continue;
-        }
-        const size_t bytes = is_bias ? n * 4 : span;
+        if (!src) continue;
         if (reinterpret_cast<uintptr_t>(src) & 3)
             return set_error(ZKML_ERR_INVALID_ARG, "weight or bias is not aligned to words");
         cudaPointerAttributes attr;
@@ -126,27 +122,39 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
         }
         if (attr.type == cudaMemoryTypeDevice && attr.device != ctx->device)
             return set_error(ZKML_ERR_INVALID_ARG, "input pointer is device memory of another GPU");
-        const uint32_t* dev = src;
-        if (attr.type != cudaMemoryTypeDevice && attr.type != cudaMemoryTypeManaged) {
-            if (drop.stage.ptr) ZK_CUDA(cudaStreamSynchronize(s));
-            if ((rc = drop.stage.ensure(bytes))) return rc;
-            ZK_CUDA(cudaMemcpyAsync(drop.stage.ptr, src, bytes, cudaMemcpyHostToDevice, s));
-            ctx->h2d_bytes += bytes;
-            dev = drop.stage.as<uint32_t>();
+        uint32_t** to = const_cast<uint32_t**>(&dev[is_bias ? 2 + g - parts : g]);
+        if (attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged) {
+            *to = const_cast<uint32_t*>(src);
+            continue;
         }
-        if (is_bias)
-            launch_linear_lay_out(dev, 1, (uint32_t)n, n, 1, lin->bias.as<uint32_t>(), (size_t)parts * n,
-                                  (size_t)(g - parts) * n, lin->status.as<uint32_t>(), s);
-        else
-            launch_linear_lay_out(dev, (uint32_t)k, (uint32_t)n, rs, cs, lin->w.as<uint32_t>(), (size_t)parts * n,
-                                  (size_t)g * n, lin->status.as<uint32_t>(), s);
-        ctx->launches++;
+        const size_t bytes = is_bias ? n * 4 : ((k - 1) * rs + (n - 1) * cs + 1) * 4;
+        if ((rc = drop.stage[g].ensure(bytes))) return rc;
+        ZK_CUDA(cudaMemcpyAsync(drop.stage[g].ptr, src, bytes, cudaMemcpyHostToDevice, s));
+        ctx->h2d_bytes += bytes;
+        *to = drop.stage[g].as<uint32_t>();
     }
-    ZK_CUDA(cudaGetLastError());
-    uint32_t st = 0;
-    ZK_CUDA(cudaMemcpyAsync(&st, lin->status.ptr, 4, cudaMemcpyDeviceToHost, s));
-    ZK_CUDA(cudaStreamSynchronize(s));
-    if (st) return set_error(ZKML_ERR_INVALID_ARG, "linear: weight or bias value >= 2^31 is not an M31 element");
+    if ((rc = lin->status.ensure(16)) || (rc = lin->base.ensure(2 * slots * 4)) || (rc = drop.sums.ensure(slots * 8)))
+        return rc;
+    // signed bytes in most models: pack one plane, and again with more where a value needs them
+    uint32_t st[2] = {0, 1};
+    for (w.planes = 1;; w.planes = st[1]) {
+        if ((rc = lin->tiles.ensure(plane * w.planes))) return rc;
+        ZK_CUDA(cudaMemsetAsync(lin->status.ptr, 0, 16, s));
+        ZK_CUDA(cudaMemsetAsync(drop.sums.ptr, 0, slots * 8, s));
+        launch_linear_pack(dev[0], dev[1], rs, cs, w, lin->tiles.as<uint8_t>(), drop.sums.as<unsigned long long>(),
+                           lin->status.as<uint32_t>(), s);
+        ZK_CUDA(cudaGetLastError());
+        launch_linear_base(drop.sums.as<unsigned long long>(), dev[2], dev[3], w, lin->base.as<uint32_t>(),
+                           lin->status.as<uint32_t>(), s);
+        ZK_CUDA(cudaGetLastError());
+        ctx->launches += 2;
+        ZK_CUDA(cudaMemcpyAsync(st, lin->status.ptr, 8, cudaMemcpyDeviceToHost, s));
+        ZK_CUDA(cudaStreamSynchronize(s));
+        if (st[0]) return set_error(ZKML_ERR_INVALID_ARG, "linear: weight or bias value >= 2^31 is not an M31 element");
+        if (st[1] <= w.planes) break;
+    }
+    w.tiles = lin->tiles.as<uint8_t>();
+    w.base = lin->base.as<uint32_t>();
     *out = lin;
     lin = nullptr;
     return ZKML_OK;
@@ -185,9 +193,9 @@ int zkml_linear_workspace(const zkml_linear* lin, size_t m, int x_bits, size_t* 
     if (x_bits != 8 && x_bits != 16 && x_bits != 31)
         return set_error(ZKML_ERR_INVALID_ARG, "x_bits must be 8, 16 or 31");
     if (m == 0) return set_error(ZKML_ERR_INVALID_ARG, "empty matrix");
-    if (m > (1u << 30) || m * lin->k > ((size_t)1 << 34) || m * lin->n > ((size_t)1 << 34))
+    if (m > (1u << 30) || m * lin->w.k > ((size_t)1 << 34) || m * lin->w.n > ((size_t)1 << 34))
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
-    *out_bytes = 0;
+    *out_bytes = linear_plan(lin->w, (uint32_t)m, x_bits, lin->ctx->num_sms).bytes;
     return ZKML_OK;
 }
 
@@ -196,12 +204,12 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     size_t need = 0;
     int rc = zkml_linear_workspace(lin, c->m, c->x_bits, &need);
     if (rc) return rc;
-    const size_t m = c->m, k = lin->k, n = lin->n;
+    const size_t m = c->m, k = lin->w.k, n = lin->w.n;
     if (c->activation < 0 || c->activation > 5)
         return set_error(ZKML_ERR_INVALID_ARG, "activation must be 0 (none) or a type tag 1 to 5");
-    if (lin->gated && c->residual)
+    if (lin->w.gated && c->residual)
         return set_error(ZKML_ERR_INVALID_ARG, "gated weights take no residual");
-    if (!lin->gated && c->up) return set_error(ZKML_ERR_INVALID_ARG, "up is an output of gated weights only");
+    if (!lin->w.gated && c->up) return set_error(ZKML_ERR_INVALID_ARG, "up is an output of gated weights only");
     const size_t most = (size_t)1 << 34;
     if (c->ldx > most || c->ld_residual > most || c->ld_out > most || c->ld_pre > most || c->ld_up > most)
         return set_error(ZKML_ERR_INVALID_ARG, "row stride too large");
@@ -209,44 +217,42 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
         return set_error(ZKML_ERR_INVALID_ARG, "the row stride of an output is below its width");
     if (c->workspace_bytes < need || (need && !c->workspace))
         return set_error(ZKML_ERR_INVALID_ARG, "workspace of " + std::to_string(need) + " bytes wanted");
+    if (reinterpret_cast<uintptr_t>(c->workspace) & 255)
+        return set_error(ZKML_ERR_INVALID_ARG, "workspace is not aligned to 256 bytes");
     zkml_ctx* ctx = lin->ctx;
     DeviceGuard guard;
     ZK_CUDA(cudaSetDevice(ctx->device));
     if ((rc = want_device_words(ctx, c->x, "x")) || (rc = want_device_words(ctx, c->out, "out")) ||
+        (rc = want_device_words(ctx, c->workspace, "workspace")) ||
         (c->residual && (rc = want_device_words(ctx, c->residual, "residual"))) ||
         (c->pre && (rc = want_device_words(ctx, c->pre, "pre"))) ||
         (c->up && (rc = want_device_words(ctx, c->up, "up"))))
         return rc;
     const Block x{c->x, m, k, c->ldx}, res{c->residual, m, n, c->ld_residual}, out{c->out, m, n, c->ld_out};
     const Block pre{c->pre, m, n, c->ld_pre}, up{c->up, m, n, c->ld_up};
+    const Block wsp{static_cast<const uint32_t*>(c->workspace), 1, need / 4, 0};
     const bool in_place = c->residual == c->out && c->ld_residual == c->ld_out;
-    if (share(out, x) || share(pre, x) || share(up, x) || share(out, pre) || share(out, up) || share(pre, up) ||
+    if (share(wsp, x) || share(wsp, out) || share(wsp, pre) || share(wsp, up) || share(wsp, res) || share(out, x) || share(pre, x) || share(up, x) || share(out, pre) || share(out, up) || share(pre, up) ||
         (!in_place && share(out, res)) || share(pre, res))
         return set_error(ZKML_ERR_INVALID_ARG, "an output overlaps another argument");
     cudaStream_t s = c->stream ? static_cast<cudaStream_t>(c->stream) : ctx->stream;
-    LinearArgs a{};
-    a.x = c->x;
-    a.w = lin->w.as<uint32_t>();
-    a.bias = lin->bias.as<uint32_t>();
-    a.residual = c->residual;
-    a.out = c->out;
-    a.pre = c->pre;
-    a.up = c->up;
-    a.status = lin->status.as<uint32_t>();
-    a.ldx = c->ldx;
-    a.ld_res = c->ld_residual;
-    a.ld_out = c->ld_out;
-    a.ld_pre = c->ld_pre;
-    a.ld_up = c->ld_up;
-    a.m = (uint32_t)m;
-    a.k = (uint32_t)k;
-    a.n = (uint32_t)n;
-    a.x_bits = c->x_bits;
-    a.activation = c->activation;
-    a.gated = lin->gated;
-    launch_linear_simple(a, s);
-    ctx->launches++;
+    LinearIO io{};
+    io.x = c->x;
+    io.residual = c->residual;
+    io.out = c->out;
+    io.pre = c->pre;
+    io.up = c->up;
+    io.status = lin->status.as<uint32_t>();
+    io.ldx = c->ldx;
+    io.ld_res = c->ld_residual;
+    io.ld_out = c->ld_out;
+    io.ld_pre = c->ld_pre;
+    io.ld_up = c->ld_up;
+    io.m = (uint32_t)m;
+    io.activation = c->activation;
+    ZK_CUDA(launch_linear(lin->w, linear_plan(lin->w, io.m, c->x_bits, ctx->num_sms), io, c->workspace, s));
     ZK_CUDA(cudaGetLastError());
+    ctx->launches += 2;
     return ZKML_OK;
 }
 
@@ -266,6 +272,7 @@ int zkml_linear_check(zkml_linear* lin, void* stream) {
     ZK_CUDA(cudaMemsetAsync(lin->status.ptr, 0, 4, s));
     if (st & LIN_BAD_VALUE)
         return set_error(ZKML_ERR_INVALID_ARG, "linear: input value >= 2^31 is not an M31 element");
+    if (st & LIN_TIMEOUT) return set_error(ZKML_ERR_TIMEOUT, "linear: a wait inside the product kernel ran out");
     return set_error(ZKML_ERR_INVALID_ARG, "linear: an activation does not fit the declared x_bits");
 }
 

@@ -1,129 +1,639 @@
 // Forward operators: y = f(x W + b) + r and h = f(x Wg + bg) * (x Wu + bu), mod P.
+//
+// The product is an exact signed-byte product on the tensor pipe.  An activation, read as a signed
+// integer, is split into D balanced byte digits (D = 1, 2, 4 for 8-, 16- and 31-bit activations),
+// x = o + sum_i 256^i x_i with x_i in [-128, 127] and o = 128 for D > 1 (the shift makes two digits
+// cover exactly the 16-bit integers; o's share of the product is 128 times the weights' column
+// sum, laid out beside the bias).  A weight is one balanced byte, or up to four of them (planes).
+// So z = sum_{i,p} 256^(i+p) sum_t x_i[t] w_p[t] + 128 sum_t w[t] + b, every inner sum an exact
+// s8 x s8 -> s32 product: below 2^14 K, which stays in 32 bits for K <= 1023 tiles of 128; longer
+// sums are cut there and joined mod P.
+//
+// The weights are the 128-row operand and the tokens' digits the N operand (N = D x tokens), so a
+// single token fills a 16-column product and costs the weights' bytes, nothing more, and the D
+// digits of a token meet in one thread's registers when the accumulators are read back.  Work is
+// counted in units of one 128 x 128-byte weight tile; the tiles that do not make a whole wave are
+// cut into even shares of units, one per block, and a tile's last block to finish joins its parts.
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
 #include "activation_device.cuh"
+#include "imma.cuh"
 #include "linear.cuh"
-#include "qm31.cuh"
+#include "round_arith.cuh"
+#include "tcgen05.cuh"
 
 namespace zk {
 
 namespace {
 
-// Canonical f(v); tag 0 is the identity.
-__device__ __forceinline__ uint32_t activate(int tag, uint32_t v) {
-    return tag == 0 ? v : red32(act_value(tag, v));
+constexpr uint32_t KSEG = 1023;  // K tiles per 32-bit accumulation: 1023 * 128 * 2^14 < 2^31
+
+// ---------------------------------------------------------------------------
+// Weights
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ int planes_needed(int v) {
+    if (v >= -128 && v <= 127) return 1;
+    if (v >= -32896 && v <= 32639) return 2;          // 127 * 257 and -128 * 257
+    if (v >= -8421504 && v <= 8355711) return 3;      // times 65793
+    return 4;
 }
 
-__global__ void lay_out_kernel(const uint32_t* __restrict__ src, uint32_t k, uint32_t n, size_t rs, size_t cs,
-                               uint32_t* __restrict__ dst, size_t ld, size_t off, uint32_t* __restrict__ status) {
+// One block per weight tile; a thread packs 16 consecutive K of one row per step (reads along the
+// rows of a row-major matrix are coalesced over the lanes, each store is one 16-byte chunk).
+__global__ void __launch_bounds__(256) linear_pack_kernel(const uint32_t* __restrict__ w, const uint32_t* __restrict__ w2,
+                                                          size_t rs, size_t cs, PackedWeights p,
+                                                          uint8_t* __restrict__ tiles,
+                                                          unsigned long long* __restrict__ sums,
+                                                          uint32_t* __restrict__ status) {
+    const uint32_t nt = blockIdx.x / p.k_tiles, kt = blockIdx.x % p.k_tiles;
     uint32_t bad = 0;
-    const size_t total = (size_t)k * n;
-    for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < total; i += (size_t)gridDim.x * blockDim.x) {
-        const size_t r = i / n, c = i % n;
-        const uint32_t v = src[r * rs + c * cs];
-        bad |= v >> 31;
-        dst[r * ld + off + c] = red32(v);
+    int need = 1;
+    for (uint32_t e = threadIdx.x; e < LIN_ROWS * 8; e += 256) {
+        const uint32_t r = e % LIN_ROWS, c = e / LIN_ROWS;
+        const uint32_t part = p.gated ? (r >> 4) & 1 : 0;
+        const uint32_t f = p.gated ? nt * 64 + (r >> 5) * 16 + (r & 15) : nt * LIN_ROWS + r;
+        const uint32_t* src = part ? w2 : w;
+        const uint32_t k0 = kt * LIN_KB + 16 * c;
+        uint32_t d[4][4] = {};
+        unsigned long long sum = 0;
+        if (f < p.n) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                uint32_t v = k0 + i < p.k ? __ldg(src + (size_t)(k0 + i) * rs + (size_t)f * cs) : 0u;
+                bad |= v >> 31;
+                int q = m31_signed(v);
+                sum += (unsigned long long)(q < 0 ? q + (int)P : q);
+                need = max(need, planes_needed(q));
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const int g = sdigit(q);
+                    d[b][i >> 2] |= (uint32_t)(uint8_t)g << (8 * (i & 3));
+                    q = (q - g) >> 8;
+                }
+            }
+        }
+        const size_t plane = (size_t)p.n_tiles * p.k_tiles * LIN_TILE_BYTES;
+        uint8_t* dst = tiles + ((size_t)nt * p.k_tiles + kt) * LIN_TILE_BYTES + r * LIN_KB + ((c ^ (r & 7)) << 4);
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+            if (b < (int)p.planes) *reinterpret_cast<uint4*>(dst + b * plane) = make_uint4(d[b][0], d[b][1], d[b][2], d[b][3]);
+        if (sum) atomicAdd(sums + (size_t)nt * LIN_ROWS + r, sum);
     }
     if (bad) atomicOr(status, LIN_BAD_VALUE);
+    if (need > 1) atomicMax(status + 1, (uint32_t)need);
 }
 
-// 64 x 64 outputs per 256-thread block, 4 x 4 per thread, K in steps of 16 through shared memory;
-// 64-bit sums reduced every four products (4 P^2 + 2^34 < 2^64).  G = 2: both projections of the
-// gated block in one pass over x.
-template <int G>
-__global__ void __launch_bounds__(256) linear_simple_kernel(LinearArgs a) {
-    __shared__ uint32_t As[16][65];
-    __shared__ uint32_t Bs[G][16][64];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const uint32_t row0 = blockIdx.y * 64, col0 = blockIdx.x * 64;
-    const size_t ldw = (size_t)G * a.n;
-    unsigned long long acc[G][4][4] = {};
+__global__ void linear_base_kernel(const unsigned long long* __restrict__ sums, const uint32_t* __restrict__ bias,
+                                   const uint32_t* __restrict__ bias2, PackedWeights p, uint32_t* __restrict__ base,
+                                   uint32_t* __restrict__ status) {
+    const uint32_t slots = p.n_tiles * LIN_ROWS, i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= slots) return;
+    const uint32_t nt = i / LIN_ROWS, r = i % LIN_ROWS, part = p.gated ? (r >> 4) & 1 : 0;
+    const uint32_t f = p.gated ? nt * 64 + (r >> 5) * 16 + (r & 15) : i;
+    const uint32_t* src = part ? bias2 : bias;
+    const uint32_t b = src && f < p.n ? src[f] : 0u;
+    if (b >> 31) atomicOr(status, LIN_BAD_VALUE);
+    base[i] = red32(b);
+    base[slots + i] = madd(red32(b), mmul(128, red64(sums[i])));
+}
+
+// ---------------------------------------------------------------------------
+// Activations -> digit tiles
+// ---------------------------------------------------------------------------
+
+// Digit tile of (m tile, K tile): N = D x tokens rows of 128 bytes in the weights' swizzle, row
+// i x tokens + t the digit i of token t.  One block per tile; a thread takes 16 K of one token.
+// Block 0 also zeroes the counters of the cut tiles.
+template <int D>
+__global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* __restrict__ x, size_t ldx, uint32_t m,
+                                                            uint32_t k, uint32_t k_tiles, uint32_t tokens,
+                                                            uint8_t* __restrict__ out, uint32_t* __restrict__ counters,
+                                                            uint32_t n_counters, uint32_t* __restrict__ status) {
+    grid_dependents_launch();
+    if (blockIdx.x == 0)
+        for (uint32_t i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
+    const uint32_t mt = blockIdx.x / k_tiles, kt = blockIdx.x % k_tiles;
+    uint8_t* tile = out + (size_t)blockIdx.x * (D * tokens * LIN_KB);
+    const bool vec = (ldx % 4 == 0) && ((reinterpret_cast<uintptr_t>(x) & 15) == 0);
     uint32_t bad = 0;
-    const uint32_t half = a.x_bits == 31 ? 0x40000000u : 1u << (a.x_bits - 1);
-    for (uint32_t l0 = 0; l0 < a.k; l0 += 16) {
-        for (int e = threadIdx.x; e < 16 * 64; e += 256) {
-            const int rr = e / 16, ll = e % 16;
-            const uint32_t gi = row0 + rr, gl = l0 + ll;
-            uint32_t v = 0;
-            if (gi < a.m && gl < a.k) {
-                v = a.x[(size_t)gi * a.ldx + gl];
-                bad |= (v >> 31) ? LIN_BAD_VALUE : 0u;
-                v = red32(v);
-                // signed value in [-half, half)
-                if (a.x_bits != 31 && !(v < half || v >= P - half)) bad |= LIN_BAD_RANGE;
+    for (uint32_t e = threadIdx.x; e < tokens * 8; e += blockDim.x) {
+        const uint32_t t = e / 8, c = e % 8, row = mt * tokens + t, k0 = kt * LIN_KB + 16 * c;
+        uint32_t v[16];
+        const uint32_t* src = x + (size_t)row * ldx + k0;
+        if (row < m && vec && k0 + 16 <= k) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint4 q = __ldg(reinterpret_cast<const uint4*>(src) + i);
+                v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
             }
-            As[ll][rr] = v;
-            const int bl = e / 64, bc = e % 64;
-            const uint32_t gbl = l0 + bl, gbc = col0 + bc;
+        } else {
 #pragma unroll
-            for (int g = 0; g < G; g++)
-                Bs[g][bl][bc] = (gbl < a.k && gbc < a.n) ? a.w[gbl * ldw + (size_t)g * a.n + gbc] : 0u;
+            for (int i = 0; i < 16; i++) v[i] = (row < m && k0 + i < k) ? __ldg(src + i) : 0u;
         }
-        __syncthreads();
+        uint32_t d[D][4] = {};
 #pragma unroll
-        for (int ll = 0; ll < 16; ll++) {
+        for (int i = 0; i < 16; i++) {
+            if (v[i] >> 31) bad |= LIN_BAD_VALUE;
+            int q = m31_signed(v[i]) - (D > 1 ? 128 : 0);
 #pragma unroll
-            for (int g = 0; g < G; g++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        acc[g][i][j] += (unsigned long long)As[ll][ty * 4 + i] * Bs[g][ll][tx * 4 + j];
-            if ((ll & 3) == 3) {
-#pragma unroll
-                for (int g = 0; g < G; g++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) acc[g][i][j] = (acc[g][i][j] & P) + (acc[g][i][j] >> 31);
+            for (int b = 0; b < D; b++) {
+                const int g = sdigit(q);
+                d[b][i >> 2] |= (uint32_t)(uint8_t)g << (8 * (i & 3));
+                q = (q - g) >> 8;
             }
+            if (D < 4 && q != 0) bad |= LIN_BAD_RANGE;
         }
-        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < D; b++) {
+            const uint32_t r = b * tokens + t;
+            *reinterpret_cast<uint4*>(tile + r * LIN_KB + ((c ^ (r & 7)) << 4)) =
+                make_uint4(d[b][0], d[b][1], d[b][2], d[b][3]);
+        }
     }
-    if (bad) atomicOr(a.status, bad);
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t r = row0 + ty * 4 + i, c = col0 + tx * 4 + j;
-            if (r >= a.m || c >= a.n) continue;
-            uint32_t z[G];
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                z[g] = red64(acc[g][i][j]);
-                if (a.bias) z[g] = madd(z[g], a.bias[(size_t)g * a.n + c]);
+    if (bad) atomicOr(status, bad);
+}
+
+// ---------------------------------------------------------------------------
+// Product and epilogue
+// ---------------------------------------------------------------------------
+
+struct KernelArgs {
+    PackedWeights w;
+    LinearIO io;
+    const uint8_t* digits;
+    uint32_t* counters;
+    uint32_t* slots;
+    const uint32_t* base;  // bias with the digits' offset share
+    uint32_t tokens, m_tiles, tiles, sk_tiles, stages, slots_per_cta;
+};
+
+// A run of units of one tile and plane: one 32-bit accumulation.
+struct Segment {
+    uint32_t tile, plane, kt, len;
+    bool first, last, whole, head;  // of its piece (a block's share of a tile); head: the piece begins inside the tile
+    uint32_t piece_units;
+};
+
+// The segments of one block, in order: its even share of the cut tiles, then whole tiles.  All
+// roles walk the same sequence.
+struct Schedule {
+    uint32_t k_tiles, per_tile, tiles, dp;
+    uint64_t pos, sk_end;
+    uint32_t tile, at, piece_begin, piece_end;
+
+    __device__ __forceinline__ void init(const KernelArgs& a) {
+        k_tiles = a.w.k_tiles;
+        per_tile = a.w.planes * k_tiles;
+        tiles = a.tiles;
+        const uint64_t units = (uint64_t)a.sk_tiles * per_tile;
+        pos = units * blockIdx.x / gridDim.x;
+        sk_end = units * (blockIdx.x + 1) / gridDim.x;
+        dp = a.sk_tiles + blockIdx.x;
+        at = piece_begin = piece_end = 0;
+    }
+    __device__ __forceinline__ bool next(Segment& s) {
+        if (at == piece_end) {
+            if (pos < sk_end) {
+                tile = (uint32_t)(pos / per_tile);
+                const uint64_t begin = (uint64_t)tile * per_tile;
+                piece_begin = (uint32_t)(pos - begin);
+                piece_end = (uint32_t)min((uint64_t)per_tile, sk_end - begin);
+                pos = begin + piece_end;
+            } else if (dp < tiles) {
+                tile = dp;
+                piece_begin = 0;
+                piece_end = per_tile;
+                dp += gridDim.x;
+            } else {
+                return false;
             }
-            if (a.pre) a.pre[(size_t)r * a.ld_pre + c] = z[0];
-            uint32_t y = activate(a.activation, z[0]);
-            if (G == 2) {
-                if (a.up) a.up[(size_t)r * a.ld_up + c] = z[G - 1];
-                y = mmul(y, z[G - 1]);
-            } else if (a.residual) {
-                const uint32_t v = a.residual[(size_t)r * a.ld_res + c];
-                if (v >> 31) atomicOr(a.status, LIN_BAD_VALUE);
-                y = madd(y, red32(v));
-            }
-            a.out[(size_t)r * a.ld_out + c] = y;
+            at = piece_begin;
         }
+        s.tile = tile;
+        s.plane = at / k_tiles;
+        s.kt = at - s.plane * k_tiles;
+        s.len = min(min(piece_end - at, k_tiles - s.kt), KSEG);
+        s.first = at == piece_begin;
+        at += s.len;
+        s.last = at == piece_end;
+        s.whole = piece_begin == 0 && piece_end == per_tile;
+        s.head = piece_begin != 0;
+        s.piece_units = piece_end - piece_begin;
+        return true;
+    }
+};
+
+// Tiles in groups of up to 8 m tiles, the m tiles of a group innermost, so that blocks running at
+// the same time share weight and digit tiles in L2.
+__device__ __forceinline__ void tile_at(const KernelArgs& a, uint32_t tile, uint32_t& mt, uint32_t& nt) {
+    const uint32_t per_group = 8 * a.w.n_tiles, group = tile / per_group, i = tile - group * per_group;
+    const uint32_t high = min(8u, a.m_tiles - 8 * group);
+    nt = i / high;
+    mt = 8 * group + i - nt * high;
+}
+
+// f(v), canonical.  Where SiLU and GELU equal their argument or round to zero in binary64 the
+// result is taken without evaluating them: for real x >= 37, exp(-x) < 2^-53 and 1 + exp(-x) is
+// 1; for x <= -16, |x| exp(x) 2^16 < 1/2; for |x| >= 8.5, |tanh| of GELU's inner term (above 28)
+// is 1.
+__device__ __forceinline__ uint32_t activate(int tag, uint32_t v) {
+    if (tag == 0) return v;
+    if (tag == 1) return v <= (P - 1) / 2 ? v : 0u;
+    if (tag == 5 || tag == 2) {
+        const bool neg = v > (P - 1) / 2;
+        const uint32_t mag = neg ? P - v : v;
+        const uint32_t sat = tag == 2 ? (17u << 15) : neg ? (16u << 16) : (37u << 16);
+        if (mag >= sat) return neg ? 0u : v;
+    }
+    return red32(act_value(tag, v));
+}
+
+// Tokens handled together: their digits are 16 accumulator columns.
+template <int D>
+constexpr int GROUP = 16 / D;
+
+// sum_i 256^i acc_i mod P of one token's accumulators.
+template <int D>
+__device__ __forceinline__ uint32_t join_digits(const uint32_t (&r)[16], int t) {
+    if (D == 1) {
+        const int v = (int)r[t];
+        return red32(v < 0 ? (uint32_t)(v + 0x7fffffff) : (uint32_t)v);
+    }
+    int64_t s = 0;
+#pragma unroll
+    for (int i = D - 1; i >= 0; i--) s = s * 256 + (int)r[i * GROUP<D> + t];
+    return canon64((uint64_t)s + ((uint64_t)P << 26));  // |s| < 2^56
+}
+
+// Finishes GROUP tokens of this lane's row: z (without the bias) -> outputs.
+template <int D, bool GATED>
+__device__ __forceinline__ void finish_tokens(const KernelArgs& a, uint32_t nt, uint32_t row, uint32_t tok0,
+                                              uint32_t base, uint32_t (&z)[GROUP<D>]) {
+    const LinearIO& io = a.io;
+    constexpr int G = GROUP<D>;
+#pragma unroll
+    for (int t = 0; t < G; t++) z[t] = madd(z[t], base);
+    if (GATED) {
+        // lane l < 16: gate, lane l + 16: up of the same output; of each token pair one lane
+        // finishes the first token and the other the second
+        const bool up_lane = (row & 16) != 0;
+        const uint32_t f = nt * 64 + (row >> 5) * 16 + (row & 15);
+#pragma unroll
+        for (int t = 0; t < G; t += 2) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up_lane ? z[t] : z[t + 1], 16);
+            const uint32_t g = up_lane ? got : z[t], u = up_lane ? z[t + 1] : got;
+            const uint32_t tok = tok0 + t + (up_lane ? 1 : 0);
+            if (f < a.w.n && tok < io.m) {
+                if (io.pre) io.pre[(size_t)tok * io.ld_pre + f] = g;
+                if (io.up) io.up[(size_t)tok * io.ld_up + f] = u;
+                io.out[(size_t)tok * io.ld_out + f] = mmul(activate(io.activation, g), u);
+            }
+        }
+    } else {
+        const uint32_t f = nt * LIN_ROWS + row;
+        if (f >= a.w.n) return;
+        uint32_t res[G], bad = 0;
+#pragma unroll
+        for (int t = 0; t < G; t++) res[t] = io.residual && tok0 + t < io.m ? io.residual[(size_t)(tok0 + t) * io.ld_res + f] : 0u;
+#pragma unroll
+        for (int t = 0; t < G; t++) {
+            if (tok0 + t >= io.m) continue;
+            if (io.pre) io.pre[(size_t)(tok0 + t) * io.ld_pre + f] = z[t];
+            bad |= res[t] >> 31;
+            io.out[(size_t)(tok0 + t) * io.ld_out + f] = madd(activate(io.activation, z[t]), red32(res[t]));
+        }
+        if (bad) atomicOr(io.status, LIN_BAD_VALUE);
+    }
+}
+
+// Whether `ok` holds in all 128 epilogue threads: they go on, or give up, together.
+__device__ __forceinline__ bool all_of_epilogue(bool ok) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+        : "=r"(r)
+        : "r"((uint32_t)ok)
+        : "memory");
+    return r != 0;
+}
+
+template <int D, bool GATED>
+__global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ KernelArgs a) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * 16 + 5];
+    __shared__ uint32_t tmem_base_s, last_s;
+    __shared__ volatile uint32_t quit_s;
+    constexpr int G = GROUP<D>;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t n_cols = D * a.tokens, b_bytes = n_cols * LIN_KB, stage_bytes = LIN_TILE_BYTES + b_bytes;
+    const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
+    const uint32_t full = smem_addr(bars), empty = full + 8 * 16, acc_full = empty + 8 * 16, acc_empty = acc_full + 16;
+    const uint32_t drained = acc_empty + 16;
+    uint32_t cols = 32;
+    while (cols < 2 * n_cols) cols <<= 1;
+    if (threadIdx.x == 0) {
+        quit_s = 0;
+        for (uint32_t i = 0; i < a.stages; i++) {
+            mbar_init(full + 8 * i, 1);
+            mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(acc_full + 8 * i, 1);
+            mbar_init(acc_empty + 8 * i, 128);
+        }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) tmem_alloc(smem_addr(&tmem_base_s), cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- loads: the weight tiles of the first stages do not wait for the digit kernel
+            Schedule sch;
+            sch.init(a);
+            Segment s{};
+            const uint8_t* wp = nullptr;
+            const uint8_t* xp = nullptr;
+            uint32_t left = 0;
+            auto advance = [&]() {  // next unit's pointers
+                if (left == 0) {
+                    if (!sch.next(s)) return false;
+                    uint32_t mt, nt;
+                    tile_at(a, s.tile, mt, nt);
+                    wp = a.w.tiles + (((size_t)s.plane * a.w.n_tiles + nt) * a.w.k_tiles + s.kt) * LIN_TILE_BYTES;
+                    xp = a.digits + ((size_t)mt * a.w.k_tiles + s.kt) * b_bytes;
+                    left = s.len;
+                } else {
+                    wp += LIN_TILE_BYTES;
+                    xp += b_bytes;
+                }
+                left--;
+                return true;
+            };
+            const uint8_t* first_x[16];
+            uint32_t issued = 0;
+            bool more = true;
+#pragma unroll
+            for (uint32_t i = 0; i < 16; i++) {
+                if (i >= a.stages || !(more = advance())) break;
+                first_x[i] = xp;
+                mbar_expect_tx(full + 8 * i, stage_bytes);
+                bulk_load(smem0 + i * stage_bytes, wp, LIN_TILE_BYTES, full + 8 * i);
+                issued++;
+            }
+            grid_dependency_wait();
+#pragma unroll
+            for (uint32_t i = 0; i < 16; i++)
+                if (i < issued)
+                    bulk_load(smem0 + i * stage_bytes + LIN_TILE_BYTES, first_x[i], b_bytes, full + 8 * i);
+            uint32_t st = 0, phase = 0;
+            while (more && issued >= a.stages && advance()) {
+                if (!mbar_wait(empty + 8 * st, phase, &quit_s)) break;
+                mbar_expect_tx(full + 8 * st, stage_bytes);
+                bulk_load(smem0 + st * stage_bytes, wp, LIN_TILE_BYTES, full + 8 * st);
+                bulk_load(smem0 + st * stage_bytes + LIN_TILE_BYTES, xp, b_bytes, full + 8 * st);
+                issued++;
+                if (++st == a.stages) st = 0, phase ^= 1;
+            }
+            if (quit_s) {  // copies in flight land before the block ends
+                atomicOr(a.io.status, LIN_TIMEOUT);
+                volatile uint32_t never = 0;
+                for (uint32_t i = 0; i < min(issued, a.stages); i++) {
+                    const uint32_t u = issued - 1 - i;
+                    mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ---- products
+            Schedule sch;
+            sch.init(a);
+            Segment s{};
+            const uint32_t idesc = tc_idesc_s8(n_cols);
+            uint32_t st = 0, phase = 0, seg = 0;
+            bool ok = true;
+            while (ok && sch.next(s)) {
+                const uint32_t buf = seg & 1, use = seg >> 1;
+                ok = mbar_wait(acc_empty + 8 * buf, (use & 1) ^ 1, &quit_s);
+                tc_fence_after();
+                const uint32_t d = tmem + buf * (cols / 2);
+                for (uint32_t u = 0; ok && u < s.len; u++) {
+                    if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s))) break;
+                    tc_fence_after();
+                    const uint64_t da = tc_desc_k128(smem0 + st * stage_bytes);
+                    const uint64_t db = tc_desc_k128(smem0 + st * stage_bytes + LIN_TILE_BYTES);
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) tc_mma_s8(d, da + 2 * i, db + 2 * i, idesc, (u | i) != 0);
+                    tc_commit(empty + 8 * st);
+                    if (++st == a.stages) st = 0, phase ^= 1;
+                }
+                if (ok) tc_commit(acc_full + 8 * buf);
+                seg++;
+            }
+            if (!ok) {  // products in flight end before the block does
+                atomicOr(a.io.status, LIN_TIMEOUT);
+                volatile uint32_t never = 0;
+                tc_commit(drained);
+                mbar_wait(drained, 0, &never);
+            }
+        }
+    } else {
+        // ---- accumulators -> outputs; this warp's TMEM lanes are 32 (warp % 4) and up
+        grid_dependency_wait();  // the counters are zeroed by the kernel before
+        const uint32_t quad = warp & 3, row = quad * 32 + lane;
+        Schedule sch;
+        sch.init(a);
+        Segment s{};
+        uint32_t seg = 0;
+        uint32_t* const my_slots = a.slots + (size_t)blockIdx.x * a.slots_per_cta * a.tokens * LIN_ROWS;
+        while (sch.next(s)) {
+            const uint32_t buf = seg & 1, use = seg >> 1;
+            seg++;
+            if (!all_of_epilogue(mbar_wait(acc_full + 8 * buf, use & 1, &quit_s))) break;
+            tc_fence_after();
+            uint32_t mt, nt;
+            tile_at(a, s.tile, mt, nt);
+            const uint32_t acc = tmem + buf * (cols / 2) + ((quad * 32) << 16);
+            const uint32_t base = a.base[(size_t)nt * LIN_ROWS + row];
+            const bool direct = s.whole && s.last;
+            // slot: 0 a piece that begins inside its tile, 1 one that ends inside it, 2 a whole tile of several segments
+            uint32_t* slot = my_slots + (size_t)(s.whole ? 2 : s.head ? 0 : 1) * a.tokens * LIN_ROWS + row;
+            const uint32_t scale = pow256(s.plane);
+            const uint32_t live = min(a.tokens, a.io.m - mt * a.tokens);  // tokens of this tile
+            for (uint32_t t0 = 0; t0 < live; t0 += G) {
+                uint32_t r[16], z[G];
+                if (D == 1) tmem_ld16(r, acc + t0);
+#pragma unroll
+                for (int i = 0; i < D; i++) {
+                    if (D == 2) tmem_ld8(r, 8 * i, acc + i * a.tokens + t0);
+                    if (D == 4) tmem_ld4(r, 4 * i, acc + i * a.tokens + t0);
+                }
+                tmem_wait_ld();
+#pragma unroll
+                for (int t = 0; t < G; t++) {
+                    z[t] = join_digits<D>(r, t);
+                    if (s.plane) z[t] = mmul(z[t], scale);
+                }
+                if (!s.first) {
+#pragma unroll
+                    for (int t = 0; t < G; t++) z[t] = madd(z[t], slot[(size_t)(t0 + t) * LIN_ROWS]);
+                }
+                if (direct) {
+                    finish_tokens<D, GATED>(a, nt, row, mt * a.tokens + t0, base, z);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < G; t++) slot[(size_t)(t0 + t) * LIN_ROWS] = z[t];
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(acc_empty + 8 * buf);
+            if (direct || !s.last) continue;
+            // a part of a cut tile: the block that completes the tile's units joins the parts
+            __threadfence();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (threadIdx.x == 64) {
+                const uint32_t before = atomicAdd(a.counters + s.tile, s.piece_units);
+                __threadfence();
+                last_s = before + s.piece_units == sch.per_tile;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (last_s) {
+                __threadfence();
+                const uint64_t units = (uint64_t)a.sk_tiles * sch.per_tile, begin = (uint64_t)s.tile * sch.per_tile;
+                // block b holds the units from units * b / blocks on
+                const uint32_t b0 = (uint32_t)(((begin + 1) * gridDim.x - 1) / units);
+                const uint32_t b1 = (uint32_t)(((begin + sch.per_tile) * gridDim.x - 1) / units);
+                const size_t pitch = (size_t)a.slots_per_cta * a.tokens * LIN_ROWS;
+                for (uint32_t t0 = 0; t0 < live; t0 += G) {
+                    uint64_t sum[G];
+                    uint32_t z[G];
+#pragma unroll
+                    for (int t = 0; t < G; t++) sum[t] = 0;
+                    for (uint32_t b = b0; b <= b1; b++) {
+                        const uint32_t* q = a.slots + b * pitch + (size_t)(b == b0 ? 1 : 0) * a.tokens * LIN_ROWS + row;
+#pragma unroll
+                        for (int t = 0; t < G; t++) sum[t] += __ldcg(q + (size_t)(t0 + t) * LIN_ROWS);
+                    }
+#pragma unroll
+                    for (int t = 0; t < G; t++) z[t] = canon64(sum[t]);
+                    finish_tokens<D, GATED>(a, nt, row, mt * a.tokens + t0, base, z);
+                }
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");  // last_s is read before it is written again
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tmem_free(tmem, cols);
+}
+
+constexpr uint32_t SMEM_MAX = 220 * 1024;
+
+template <int D, bool GATED>
+cudaError_t configure_one() {
+    return cudaFuncSetAttribute(linear_kernel<D, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+}
+
+template <int D>
+void launch_digits(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, uint8_t* out, uint32_t* counters,
+                   cudaStream_t s) {
+    const uint32_t threads = std::min(256u, (p.tokens * 8 + 31) / 32 * 32);
+    linear_digits_kernel<D><<<p.m_tiles * w.k_tiles, threads, 0, s>>>(io.x, io.ldx, io.m, w.k, w.k_tiles, p.tokens, out,
+                                                                    counters, p.sk_tiles, io.status);
 }
 
 }  // namespace
 
-void launch_linear_lay_out(const uint32_t* src, uint32_t k, uint32_t n, size_t rs, size_t cs, uint32_t* dst,
-                           size_t ld, size_t off, uint32_t* status, cudaStream_t s) {
-    const size_t total = (size_t)k * n;
-    const unsigned g = (unsigned)std::min<size_t>((total + 255) / 256, 8192);
-    lay_out_kernel<<<g, 256, 0, s>>>(src, k, n, rs, cs, dst, ld, off, status);
+void launch_linear_pack(const uint32_t* w, const uint32_t* w2, size_t rs, size_t cs, const PackedWeights& p,
+                        uint8_t* tiles, unsigned long long* sums, uint32_t* status, cudaStream_t s) {
+    linear_pack_kernel<<<p.k_tiles * p.n_tiles, 256, 0, s>>>(w, w2, rs, cs, p, tiles, sums, status);
 }
 
-void launch_linear_simple(const LinearArgs& a, cudaStream_t s) {
-    const dim3 grid((a.n + 63) / 64, (a.m + 63) / 64);
-    if (a.gated)
-        linear_simple_kernel<2><<<grid, 256, 0, s>>>(a);
+void launch_linear_base(const unsigned long long* sums, const uint32_t* bias, const uint32_t* bias2,
+                        const PackedWeights& p, uint32_t* base, uint32_t* status, cudaStream_t s) {
+    linear_base_kernel<<<p.n_tiles, LIN_ROWS, 0, s>>>(sums, bias, bias2, p, base, status);
+}
+
+LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms) {
+    LinearPlan p{};
+    p.digits = x_bits == 8 ? 1 : x_bits == 16 ? 2 : 4;
+    const uint32_t unit = 16 / p.digits, most = 256 / p.digits;  // N = digits x tokens: a multiple of 16, at most 256
+    p.m_tiles = (m + most - 1) / most;
+    p.tokens = ((m + p.m_tiles - 1) / p.m_tiles + unit - 1) / unit * unit;
+    p.m_tiles = (m + p.tokens - 1) / p.tokens;
+    p.tiles = p.m_tiles * w.n_tiles;
+    const uint64_t per_tile = (uint64_t)w.planes * w.k_tiles, units = per_tile * p.tiles;
+    p.ctas = (uint32_t)std::min<uint64_t>((uint64_t)num_sms, units);
+    const uint32_t waves = p.tiles / p.ctas;
+    p.sk_tiles = p.tiles % p.ctas == 0 ? 0 : waves ? p.tiles - (waves - 1) * p.ctas : p.tiles;
+    const uint32_t stage = LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB;
+    p.stages = std::min(16u, (SMEM_MAX - 1024) / stage);
+    p.slots = w.planes > 1 || w.k_tiles > KSEG ? 3 : p.sk_tiles ? 2 : 0;
+    auto up = [](size_t v) { return (v + 1023) / 1024 * 1024; };
+    p.digits_off = up((size_t)p.sk_tiles * 4);
+    p.slots_off = p.digits_off + up((size_t)p.m_tiles * w.k_tiles * p.digits * p.tokens * LIN_KB);
+    p.bytes = p.slots_off + (size_t)p.ctas * p.slots * p.tokens * LIN_ROWS * 4;
+    return p;
+}
+
+cudaError_t linear_configure() {
+    cudaError_t e = configure_one<1, false>();
+    if (e == cudaSuccess) e = configure_one<2, false>();
+    if (e == cudaSuccess) e = configure_one<4, false>();
+    if (e == cudaSuccess) e = configure_one<1, true>();
+    if (e == cudaSuccess) e = configure_one<2, true>();
+    if (e == cudaSuccess) e = configure_one<4, true>();
+    return e;
+}
+
+cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, void* workspace,
+                          cudaStream_t s) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    KernelArgs a{};
+    a.w = w;
+    a.io = io;
+    a.counters = reinterpret_cast<uint32_t*>(ws);
+    a.digits = ws + p.digits_off;
+    a.slots = reinterpret_cast<uint32_t*>(ws + p.slots_off);
+    a.base = w.base + (p.digits > 1 ? (size_t)w.n_tiles * LIN_ROWS : 0);
+    a.tokens = p.tokens;
+    a.m_tiles = p.m_tiles;
+    a.tiles = p.tiles;
+    a.sk_tiles = p.sk_tiles;
+    a.stages = p.stages;
+    a.slots_per_cta = p.slots;
+    if (p.digits == 1)
+        launch_digits<1>(w, p, io, ws + p.digits_off, a.counters, s);
+    else if (p.digits == 2)
+        launch_digits<2>(w, p, io, ws + p.digits_off, a.counters, s);
     else
-        linear_simple_kernel<1><<<grid, 256, 0, s>>>(a);
+        launch_digits<4>(w, p, io, ws + p.digits_off, a.counters, s);
+    // programmatic dependent: its blocks set up and load weights while the digits are made
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.ctas);
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = p.stages * (LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB) + 1024;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (w.gated)
+        return p.digits == 1   ? cudaLaunchKernelEx(&cfg, linear_kernel<1, true>, a)
+               : p.digits == 2 ? cudaLaunchKernelEx(&cfg, linear_kernel<2, true>, a)
+                               : cudaLaunchKernelEx(&cfg, linear_kernel<4, true>, a);
+    return p.digits == 1   ? cudaLaunchKernelEx(&cfg, linear_kernel<1, false>, a)
+           : p.digits == 2 ? cudaLaunchKernelEx(&cfg, linear_kernel<2, false>, a)
+                           : cudaLaunchKernelEx(&cfg, linear_kernel<4, false>, a);
 }
 
 }  // namespace zk
