@@ -28,6 +28,11 @@ namespace zk {
 
 namespace {
 
+// Epilogue warps: four to each quarter of the accumulators' rows, taking every fourth token group.
+// One warp a quarter left each scheduler a single chain of dependent instructions and bound most
+// calls by it (64 tokens x 5120 x 13824: 58 us with 4 warps).
+constexpr uint32_t EPI_WARPS = 16, EPI_THREADS = 32 * EPI_WARPS, EPI_SUBS = EPI_WARPS / 4;
+constexpr uint32_t THREADS = 64 + EPI_THREADS;
 constexpr uint32_t KSEG = 1023;  // K tiles per 32-bit accumulation: 1023 * 128 * 2^14 < 2^31
 
 // ---------------------------------------------------------------------------
@@ -309,19 +314,19 @@ __device__ __forceinline__ void finish_tokens(const KernelArgs& a, uint32_t nt, 
     }
 }
 
-// Whether `ok` holds in all 128 epilogue threads: they go on, or give up, together.
+// Whether `ok` holds in all epilogue threads: they go on, or give up, together.
 __device__ __forceinline__ bool all_of_epilogue(bool ok) {
     uint32_t r;
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, 1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
         : "=r"(r)
-        : "r"((uint32_t)ok)
+        : "r"((uint32_t)ok), "n"(EPI_THREADS)
         : "memory");
     return r != 0;
 }
 
 template <int D, bool GATED>
-__global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ KernelArgs a) {
+__global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constant__ KernelArgs a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * 16 + 5];
     __shared__ uint32_t tmem_base_s, last_s;
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ 
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(acc_full + 8 * i, 1);
-            mbar_init(acc_empty + 8 * i, 128);
+            mbar_init(acc_empty + 8 * i, EPI_THREADS);
         }
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -448,7 +453,7 @@ __global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ 
     } else {
         // ---- accumulators -> outputs; this warp's TMEM lanes are 32 (warp % 4) and up
         grid_dependency_wait();  // the counters are zeroed by the kernel before
-        const uint32_t quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t quad = warp & 3, row = quad * 32 + lane, sub = (warp - 2) >> 2;
         Schedule sch;
         sch.init(a);
         Segment s{};
@@ -468,7 +473,7 @@ __global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ 
             uint32_t* slot = my_slots + (size_t)(s.whole ? 2 : s.head ? 0 : 1) * a.tokens * LIN_ROWS + row;
             const uint32_t scale = pow256(s.plane);
             const uint32_t live = min(a.tokens, a.io.m - mt * a.tokens);  // tokens of this tile
-            for (uint32_t t0 = 0; t0 < live; t0 += G) {
+            for (uint32_t t0 = sub * G; t0 < live; t0 += EPI_SUBS * G) {
                 uint32_t r[16], z[G];
                 if (D == 1) tmem_ld16(r, acc + t0);
 #pragma unroll
@@ -498,13 +503,13 @@ __global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ 
             if (direct || !s.last) continue;
             // a part of a cut tile: the block that completes the tile's units joins the parts
             __threadfence();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");
             if (threadIdx.x == 64) {
                 const uint32_t before = atomicAdd(a.counters + s.tile, s.piece_units);
                 __threadfence();
                 last_s = before + s.piece_units == sch.per_tile;
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");
             if (last_s) {
                 __threadfence();
                 const uint64_t units = (uint64_t)a.sk_tiles * sch.per_tile, begin = (uint64_t)s.tile * sch.per_tile;
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ 
                 const uint32_t b0 = (uint32_t)(((begin + 1) * gridDim.x - 1) / units);
                 const uint32_t b1 = (uint32_t)(((begin + sch.per_tile) * gridDim.x - 1) / units);
                 const size_t pitch = (size_t)a.slots_per_cta * a.tokens * LIN_ROWS;
-                for (uint32_t t0 = 0; t0 < live; t0 += G) {
+                for (uint32_t t0 = sub * G; t0 < live; t0 += EPI_SUBS * G) {
                     uint64_t sum[G];
                     uint32_t z[G];
 #pragma unroll
@@ -527,7 +532,7 @@ __global__ void __launch_bounds__(192, 1) linear_kernel(const __grid_constant__ 
                     finish_tokens<D, GATED>(a, nt, row, mt * a.tokens + t0, base, z);
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // last_s is read before it is written again
+            asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");  // last_s is read before it is written again
         }
     }
     tc_fence_before();
@@ -622,7 +627,7 @@ cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const Lin
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(p.ctas);
-    cfg.blockDim = dim3(192);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = p.stages * (LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB) + 1024;
     cfg.stream = s;
     cfg.attrs = &attr;
