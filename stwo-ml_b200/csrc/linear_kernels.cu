@@ -110,22 +110,23 @@ __global__ void linear_base_kernel(const unsigned long long* __restrict__ sums, 
 // ---------------------------------------------------------------------------
 
 // Digit tile of (m tile, K tile): N = D x tokens rows of 128 bytes in the weights' swizzle, row
-// i x tokens + t the digit i of token t.  One block per tile; a thread takes 16 K of one token.
-// Block 0 also zeroes the counters of the cut tiles.
+// i x tokens + t the digit i of token t.  A block takes 32 tokens of a tile (all, if fewer), a
+// thread 16 K of one token.  Block 0 also zeroes the counters of the cut tiles.
 template <int D>
 __global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* __restrict__ x, size_t ldx, uint32_t m,
                                                             uint32_t k, uint32_t k_tiles, uint32_t tokens,
                                                             uint8_t* __restrict__ out, uint32_t* __restrict__ counters,
                                                             uint32_t n_counters, uint32_t* __restrict__ status) {
     grid_dependents_launch();
-    if (blockIdx.x == 0)
+    if (blockIdx.x == 0 && blockIdx.y == 0)
         for (uint32_t i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
     const uint32_t mt = blockIdx.x / k_tiles, kt = blockIdx.x % k_tiles;
     uint8_t* tile = out + (size_t)blockIdx.x * (D * tokens * LIN_KB);
     const bool vec = (ldx % 4 == 0) && ((reinterpret_cast<uintptr_t>(x) & 15) == 0);
     uint32_t bad = 0;
-    for (uint32_t e = threadIdx.x; e < tokens * 8; e += blockDim.x) {
-        const uint32_t t = e / 8, c = e % 8, row = mt * tokens + t, k0 = kt * LIN_KB + 16 * c;
+    const uint32_t t = blockIdx.y * 32 + threadIdx.x / 8, c = threadIdx.x % 8;
+    if (t < tokens) {
+        const uint32_t row = mt * tokens + t, k0 = kt * LIN_KB + 16 * c;
         uint32_t v[16];
         const uint32_t* src = x + (size_t)row * ldx + k0;
         if (row < m && vec && k0 + 16 <= k) {
@@ -240,6 +241,41 @@ __device__ __forceinline__ void tile_at(const KernelArgs& a, uint32_t tile, uint
     mt = 8 * group + i - nt * high;
 }
 
+// SiLU or GELU of the M31 word v with |real| below the saturation bound, canonical.
+// Both are mag * w / (1 + e) in units of 2^-16, with mag = |v|, w = 1 for positive and e for
+// negative v, and e = exp(-a), a = |x| for SiLU and 2 |u| for GELU's inner term u
+// (1 + tanh u = 2 / (1 + exp(-2u))).  e = 2^-k exp(r), |r| <= ln(2) / 2, by the Taylor polynomial
+// of degree 9 (remainder below 2^-37), 1 / (1 + e) by one Newton step from a single-precision
+// estimate (below 2^-43): the result, below 2^21.3, is off by less than 2^-15.  Where it lies
+// within 2^-12 of a half-integer the defining binary64 form decides the rounding.  About 25
+// double-precision operations instead of the 150 and more of exp, tanh and a division.
+__device__ __forceinline__ uint32_t bent_activation(int tag, uint32_t v, uint32_t mag, bool neg) {
+    const double x = (double)mag * (1.0 / 65536.0);
+    double a = x;
+    if (tag == 2) a = 2.0 * 0.79788456080286535588 * fma(0.044715 * x * x, x, x);  // 2 sqrt(2 / pi) (x + 0.044715 x^3)
+    const int k = __double2int_rn(a * 1.44269504088896340736);  // a / ln 2
+    const double r = fma((double)k, 0.69314718055994530942, -a);
+    double e = 1.0 / 362880.0;
+    e = fma(e, r, 1.0 / 40320.0);
+    e = fma(e, r, 1.0 / 5040.0);
+    e = fma(e, r, 1.0 / 720.0);
+    e = fma(e, r, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    e *= __hiloint2double((1023 - k) << 20, 0);  // k < 90
+    const double d = 1.0 + e;
+    const double q0 = (double)__fdividef(1.0f, (float)d);
+    const double q = q0 * fma(-d, q0, 2.0);
+    const double y = (double)mag * (neg ? e * q : q);
+    const double whole = floor(y), rest = y - whole;
+    if (fabs(rest - 0.5) < 1.0 / 4096.0) return red32(act_value(tag, v));
+    const uint32_t n = (uint32_t)whole + (rest >= 0.5 ? 1u : 0u);
+    return neg && n ? P - n : n;
+}
+
 // f(v), canonical.  Where SiLU and GELU equal their argument or round to zero in binary64 the
 // result is taken without evaluating them: for real x >= 37, exp(-x) < 2^-53 and 1 + exp(-x) is
 // 1; for x <= -16, |x| exp(x) 2^16 < 1/2; for |x| >= 8.5, |tanh| of GELU's inner term (above 28)
@@ -252,6 +288,7 @@ __device__ __forceinline__ uint32_t activate(int tag, uint32_t v) {
         const uint32_t mag = neg ? P - v : v;
         const uint32_t sat = tag == 2 ? (17u << 15) : neg ? (16u << 16) : (37u << 16);
         if (mag >= sat) return neg ? 0u : v;
+        return bent_activation(tag, v, mag, neg);
     }
     return red32(act_value(tag, v));
 }
@@ -352,6 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();  // the block barriers want whole warps
     if (warp == 2) tmem_alloc(smem_addr(&tmem_base_s), cols);
     tc_fence_before();
     __syncthreads();
@@ -517,15 +555,26 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                 const uint32_t b0 = (uint32_t)(((begin + 1) * gridDim.x - 1) / units);
                 const uint32_t b1 = (uint32_t)(((begin + sch.per_tile) * gridDim.x - 1) / units);
                 const size_t pitch = (size_t)a.slots_per_cta * a.tokens * LIN_ROWS;
+                constexpr int PARTS = D == 1 ? 1 : D == 2 ? 2 : 4;
                 for (uint32_t t0 = sub * G; t0 < live; t0 += EPI_SUBS * G) {
                     uint64_t sum[G];
                     uint32_t z[G];
 #pragma unroll
                     for (int t = 0; t < G; t++) sum[t] = 0;
-                    for (uint32_t b = b0; b <= b1; b++) {
-                        const uint32_t* q = a.slots + b * pitch + (size_t)(b == b0 ? 1 : 0) * a.tokens * LIN_ROWS + row;
+                    for (uint32_t b = b0; b <= b1; b += PARTS) {  // PARTS parts' loads in flight together
+                        uint32_t v[PARTS][G];
 #pragma unroll
-                        for (int t = 0; t < G; t++) sum[t] += __ldcg(q + (size_t)(t0 + t) * LIN_ROWS);
+                        for (int i = 0; i < PARTS; i++) {
+                            const uint32_t* q = a.slots + (b + i) * pitch +
+                                                (size_t)(b + i == b0 ? 1 : 0) * a.tokens * LIN_ROWS +
+                                                (size_t)t0 * LIN_ROWS + row;
+#pragma unroll
+                            for (int t = 0; t < G; t++) v[i][t] = b + i <= b1 ? __ldcg(q + t * LIN_ROWS) : 0u;
+                        }
+#pragma unroll
+                        for (int i = 0; i < PARTS; i++)
+#pragma unroll
+                            for (int t = 0; t < G; t++) sum[t] += v[i][t];
                     }
 #pragma unroll
                     for (int t = 0; t < G; t++) z[t] = canon64(sum[t]);
@@ -535,6 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
             asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");  // last_s is read before it is written again
         }
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (warp == 2) tmem_free(tmem, cols);
@@ -551,7 +601,7 @@ template <int D>
 void launch_digits(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, uint8_t* out, uint32_t* counters,
                    cudaStream_t s) {
     const uint32_t threads = std::min(256u, (p.tokens * 8 + 31) / 32 * 32);
-    linear_digits_kernel<D><<<p.m_tiles * w.k_tiles, threads, 0, s>>>(io.x, io.ldx, io.m, w.k, w.k_tiles, p.tokens, out,
+    linear_digits_kernel<D><<<dim3(p.m_tiles * w.k_tiles, (p.tokens + 31) / 32), threads, 0, s>>>(io.x, io.ldx, io.m, w.k, w.k_tiles, p.tokens, out,
                                                                     counters, p.sk_tiles, io.status);
 }
 
@@ -567,18 +617,62 @@ void launch_linear_base(const unsigned long long* sums, const uint32_t* bias, co
     linear_base_kernel<<<p.n_tiles, LIN_ROWS, 0, s>>>(sums, bias, bias2, p, base, status);
 }
 
+// Clocks of a split, by a model of what bounds it: a block takes in 50 bytes a clock from L2 and
+// multiplies 128 rows x N columns x 128 K in 2 N clocks; finishing a token of a tile takes a
+// block 40 clocks, hidden under the next tile's products except for the last tile; a cut tile's
+// parts cost a round through memory (about 3000 clocks) and 15 clocks a token and part.
+static double plan_clocks(const LinearPlan& p, uint64_t per_tile) {
+    const double n_cols = (double)p.digits * p.tokens;
+    const double unit = std::max(2.0 * n_cols, (LIN_TILE_BYTES + n_cols * LIN_KB) / 50.0);
+    const double finish = 400 + 40.0 * p.tokens, tile = unit * per_tile;
+    const uint32_t whole = (p.tiles - p.sk_tiles + p.ctas - 1) / p.ctas;
+    double t = whole * std::max(tile, finish) + finish;
+    if (p.sk_tiles) {
+        const double share = (double)p.sk_tiles * per_tile / p.ctas, parts = per_tile / share + 1;
+        t += share * unit + 3000 + std::max(1.0, (double)p.sk_tiles / p.ctas) * p.tokens * (40 + 15 * parts);
+    }
+    return t;
+}
+
 LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms) {
-    LinearPlan p{};
-    p.digits = x_bits == 8 ? 1 : x_bits == 16 ? 2 : 4;
-    const uint32_t unit = 16 / p.digits, most = 256 / p.digits;  // N = digits x tokens: a multiple of 16, at most 256
-    p.m_tiles = (m + most - 1) / most;
-    p.tokens = ((m + p.m_tiles - 1) / p.m_tiles + unit - 1) / unit * unit;
-    p.m_tiles = (m + p.tokens - 1) / p.tokens;
-    p.tiles = p.m_tiles * w.n_tiles;
-    const uint64_t per_tile = (uint64_t)w.planes * w.k_tiles, units = per_tile * p.tiles;
-    p.ctas = (uint32_t)std::min<uint64_t>((uint64_t)num_sms, units);
-    const uint32_t waves = p.tiles / p.ctas;
-    p.sk_tiles = p.tiles % p.ctas == 0 ? 0 : waves ? p.tiles - (waves - 1) * p.ctas : p.tiles;
+    LinearPlan best{};
+    const uint32_t digits = x_bits == 8 ? 1 : x_bits == 16 ? 2 : 4;
+    const uint32_t unit = 16 / digits, most = 256 / digits;  // N = digits x tokens: a multiple of 16, at most 256
+    const uint64_t per_tile = (uint64_t)w.planes * w.k_tiles;
+    double best_clocks = 0;
+    const uint32_t fewest = (m + most - 1) / most;
+    uint32_t last_tokens = 0;
+    for (uint32_t want = fewest; want <= 16 * fewest; want += std::max(1u, want / 4)) {
+        LinearPlan p{};
+        p.digits = digits;
+        p.tokens = ((m + want - 1) / want + unit - 1) / unit * unit;
+        if (p.tokens == last_tokens) continue;
+        last_tokens = p.tokens;
+        p.m_tiles = (m + p.tokens - 1) / p.tokens;
+        if (want > fewest && (uint64_t)p.m_tiles * w.n_tiles > 16u * num_sms) break;
+        p.tiles = p.m_tiles * w.n_tiles;
+        const uint32_t waves = p.tiles / num_sms;
+        // whole tiles only; the tiles beyond the last full wave but one cut over all blocks; with fewer
+        // tiles than blocks, each cut into the same number of parts
+        for (int mode = 0; mode < 6; mode++) {
+            if (mode == 0) {
+                p.ctas = std::min(p.tiles, (uint32_t)num_sms);
+                p.sk_tiles = 0;
+            } else if (mode == 1) {
+                p.ctas = (uint32_t)std::min<uint64_t>((uint64_t)num_sms, per_tile * p.tiles);
+                if (p.tiles % p.ctas == 0) continue;
+                p.sk_tiles = waves ? p.tiles - (waves - 1) * p.ctas : p.tiles;
+            } else {
+                const uint32_t parts = 1u << (mode - 1);
+                if (parts > per_tile || (uint64_t)p.tiles * parts > (uint64_t)num_sms) break;
+                p.ctas = p.tiles * parts;
+                p.sk_tiles = p.tiles;
+            }
+            const double c = plan_clocks(p, per_tile);
+            if (!best.tiles || c < best_clocks) best = p, best_clocks = c;
+        }
+    }
+    LinearPlan& p = best;
     const uint32_t stage = LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB;
     p.stages = std::min(16u, (SMEM_MAX - 1024) / stage);
     p.slots = w.planes > 1 || w.k_tiles > KSEG ? 3 : p.sk_tiles ? 2 : 0;

@@ -82,6 +82,18 @@ def test_activations_at_their_bends(act, bits):
     L.same(host(Z.LinearM31(dev(w))(dev(x), activation=act)), y, unsure)
 
 
+@pytest.mark.parametrize("act,first", [("silu", i << 20) for i in range(-2, 3)] + [("gelu", -(1 << 20)), ("gelu", 0)])
+def test_every_word_where_the_function_bends(act, first):
+    """2^20 consecutive words at a time: SiLU bends for reals in (-16, 37), GELU in (-8.5, 8.5).  Left out
+    are the words whose binary64 value lies within 2^-19 of a half-integer: 2^-18 of them, 4 expected."""
+    z = L.words(first + np.arange(1 << 20))
+    y, unsure = L.activation(z, TAGS[act])
+    assert unsure.sum() < 40
+    got = host(Z.LinearM31(dev(z.reshape(1, -1)))(torch.ones(1, 1, dtype=torch.int32, device="cuda"),
+                                                  activation=act)).reshape(-1).astype(np.int64)
+    assert ((got == y) | unsure).all()
+
+
 @pytest.mark.parametrize("x_bits,w_bits,keep,bias", [(31, 8, True, False), (8, 8, True, True), (16, 8, False, True),
                                                      (31, 31, True, True)])
 @pytest.mark.parametrize("m,k,n", [(1, 64, 1), (1, 576, 200), (3, 130, 63), (33, 257, 65), (70, 128, 129), (140, 96, 64)])
