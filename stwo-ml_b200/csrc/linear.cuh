@@ -62,7 +62,9 @@ struct LinearPlan {
 };
 LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms);
 cudaError_t linear_configure();  // per device, before the first launch
+// overlap: the weights were in place before the work now queued on s, so they may be read while
+// that work still runs.
 cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, void* workspace,
-                          cudaStream_t s);
+                          cudaStream_t s, bool overlap);
 
 }  // namespace zk

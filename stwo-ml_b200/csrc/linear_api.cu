@@ -250,7 +250,7 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     io.ld_up = c->ld_up;
     io.m = (uint32_t)m;
     io.activation = c->activation;
-    ZK_CUDA(launch_linear(lin->w, linear_plan(lin->w, io.m, c->x_bits, ctx->num_sms), io, c->workspace, s));
+    ZK_CUDA(launch_linear(lin->w, linear_plan(lin->w, io.m, c->x_bits, ctx->num_sms), io, c->workspace, s, true));
     ZK_CUDA(cudaGetLastError());
     ctx->launches += 2;
     return ZKML_OK;

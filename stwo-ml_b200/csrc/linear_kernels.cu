@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* __re
                                                             uint32_t k, uint32_t k_tiles, uint32_t tokens,
                                                             uint8_t* __restrict__ out, uint32_t* __restrict__ counters,
                                                             uint32_t n_counters, uint32_t* __restrict__ status) {
-    grid_dependents_launch();
+    grid_dependents_launch();  // the product kernel sets up and loads weights meanwhile
+    grid_dependency_wait();    // x, and the workspace's last use
     if (blockIdx.x == 0 && blockIdx.y == 0)
         for (uint32_t i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
     const uint32_t mt = blockIdx.x / k_tiles, kt = blockIdx.x % k_tiles;
@@ -364,6 +365,7 @@ __device__ __forceinline__ bool all_of_epilogue(bool ok) {
 
 template <int D, bool GATED>
 __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constant__ KernelArgs a) {
+    grid_dependents_launch();  // the next call's digit kernel, which waits for this grid's end, may take its place
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * 16 + 5];
     __shared__ uint32_t tmem_base_s, last_s;
@@ -597,12 +599,35 @@ cudaError_t configure_one() {
     return cudaFuncSetAttribute(linear_kernel<D, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
 }
 
+// Both kernels of a call are programmatic dependents: a block of the product kernel starts, and
+// loads weights, as soon as an SM is free, before the digits are made and before the last blocks
+// of the previous call are done; what depends on earlier work comes after grid_dependency_wait.
+struct Launch {
+    cudaLaunchAttribute attr{};
+    cudaLaunchConfig_t cfg{};
+    Launch(dim3 grid, unsigned block, size_t smem, cudaStream_t s, bool overlap) {
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(block);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = s;
+        cfg.attrs = &attr;
+        cfg.numAttrs = overlap ? 1 : 0;
+    }
+};
+
 template <int D>
-void launch_digits(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, uint8_t* out, uint32_t* counters,
-                   cudaStream_t s) {
-    const uint32_t threads = std::min(256u, (p.tokens * 8 + 31) / 32 * 32);
-    linear_digits_kernel<D><<<dim3(p.m_tiles * w.k_tiles, (p.tokens + 31) / 32), threads, 0, s>>>(io.x, io.ldx, io.m, w.k, w.k_tiles, p.tokens, out,
-                                                                    counters, p.sk_tiles, io.status);
+cudaError_t launch_all(const KernelArgs& a, const LinearPlan& p, uint8_t* digits, cudaStream_t s, bool overlap) {
+    const PackedWeights& w = a.w;
+    const unsigned threads = std::min(256u, (p.tokens * 8 + 31) / 32 * 32);
+    const Launch d(dim3(p.m_tiles * w.k_tiles, (p.tokens + 31) / 32), threads, 0, s, overlap);
+    cudaError_t e = cudaLaunchKernelEx(&d.cfg, linear_digits_kernel<D>, a.io.x, a.io.ldx, a.io.m, w.k, w.k_tiles,
+                                       p.tokens, digits, a.counters, p.sk_tiles, a.io.status);
+    if (e != cudaSuccess) return e;
+    const Launch l(dim3(p.ctas), THREADS, p.stages * (LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB) + 1024, s, overlap);
+    return w.gated ? cudaLaunchKernelEx(&l.cfg, linear_kernel<D, true>, a)
+                   : cudaLaunchKernelEx(&l.cfg, linear_kernel<D, false>, a);
 }
 
 }  // namespace
@@ -694,7 +719,7 @@ cudaError_t linear_configure() {
 }
 
 cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, void* workspace,
-                          cudaStream_t s) {
+                          cudaStream_t s, bool overlap) {
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     KernelArgs a{};
     a.w = w;
@@ -709,30 +734,10 @@ cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const Lin
     a.sk_tiles = p.sk_tiles;
     a.stages = p.stages;
     a.slots_per_cta = p.slots;
-    if (p.digits == 1)
-        launch_digits<1>(w, p, io, ws + p.digits_off, a.counters, s);
-    else if (p.digits == 2)
-        launch_digits<2>(w, p, io, ws + p.digits_off, a.counters, s);
-    else
-        launch_digits<4>(w, p, io, ws + p.digits_off, a.counters, s);
-    // programmatic dependent: its blocks set up and load weights while the digits are made
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.ctas);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = p.stages * (LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB) + 1024;
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (w.gated)
-        return p.digits == 1   ? cudaLaunchKernelEx(&cfg, linear_kernel<1, true>, a)
-               : p.digits == 2 ? cudaLaunchKernelEx(&cfg, linear_kernel<2, true>, a)
-                               : cudaLaunchKernelEx(&cfg, linear_kernel<4, true>, a);
-    return p.digits == 1   ? cudaLaunchKernelEx(&cfg, linear_kernel<1, false>, a)
-           : p.digits == 2 ? cudaLaunchKernelEx(&cfg, linear_kernel<2, false>, a)
-                           : cudaLaunchKernelEx(&cfg, linear_kernel<4, false>, a);
+    uint8_t* digits = ws + p.digits_off;
+    return p.digits == 1   ? launch_all<1>(a, p, digits, s, overlap)
+           : p.digits == 2 ? launch_all<2>(a, p, digits, s, overlap)
+                           : launch_all<4>(a, p, digits, s, overlap);
 }
 
 }  // namespace zk
