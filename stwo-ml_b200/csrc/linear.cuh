@@ -61,6 +61,17 @@ struct LinearPlan {
     size_t digits_off, slots_off, bytes;  // workspace: counters, digit tiles, slots
 };
 LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms);
+// The few-token kernel's split, when it takes the call: one launch, no workspace.
+struct TokenPlan {
+    uint32_t digits, tokens;
+    uint32_t parts;   // blocks of a cluster, each with a share of K
+    uint32_t stages;
+    uint32_t smem;
+};
+bool linear_token_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms, TokenPlan* out);
+cudaError_t launch_linear_token(const PackedWeights& w, const TokenPlan& p, const LinearIO& io, cudaStream_t s,
+                                bool overlap);
+cudaError_t linear_token_configure();
 cudaError_t linear_configure();  // per device, before the first launch
 // overlap: the weights were in place before the work now queued on s, so they may be read while
 // that work still runs.

@@ -86,6 +86,7 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     if (cap != cudaStreamCaptureStatusNone)
         return set_error(ZKML_ERR_INVALID_ARG, "weights cannot be laid out while the stream is captured");
     ZK_CUDA(linear_configure());
+    ZK_CUDA(linear_token_configure());
     zkml_linear* lin = new zkml_linear();
     struct Drop {
         zkml_linear*& l;
@@ -195,6 +196,9 @@ int zkml_linear_workspace(const zkml_linear* lin, size_t m, int x_bits, size_t* 
     if (m == 0) return set_error(ZKML_ERR_INVALID_ARG, "empty matrix");
     if (m > (1u << 30) || m * lin->w.k > ((size_t)1 << 34) || m * lin->w.n > ((size_t)1 << 34))
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
+    TokenPlan t;
+    *out_bytes = 0;
+    if (linear_token_plan(lin->w, (uint32_t)m, x_bits, lin->ctx->num_sms, &t)) return ZKML_OK;
     *out_bytes = linear_plan(lin->w, (uint32_t)m, x_bits, lin->ctx->num_sms).bytes;
     return ZKML_OK;
 }
@@ -217,20 +221,20 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
         return set_error(ZKML_ERR_INVALID_ARG, "the row stride of an output is below its width");
     if (c->workspace_bytes < need || (need && !c->workspace))
         return set_error(ZKML_ERR_INVALID_ARG, "workspace of " + std::to_string(need) + " bytes wanted");
-    if (reinterpret_cast<uintptr_t>(c->workspace) & 255)
+    if (need && (reinterpret_cast<uintptr_t>(c->workspace) & 255))
         return set_error(ZKML_ERR_INVALID_ARG, "workspace is not aligned to 256 bytes");
     zkml_ctx* ctx = lin->ctx;
     DeviceGuard guard;
     ZK_CUDA(cudaSetDevice(ctx->device));
     if ((rc = want_device_words(ctx, c->x, "x")) || (rc = want_device_words(ctx, c->out, "out")) ||
-        (rc = want_device_words(ctx, c->workspace, "workspace")) ||
+        (need && (rc = want_device_words(ctx, c->workspace, "workspace"))) ||
         (c->residual && (rc = want_device_words(ctx, c->residual, "residual"))) ||
         (c->pre && (rc = want_device_words(ctx, c->pre, "pre"))) ||
         (c->up && (rc = want_device_words(ctx, c->up, "up"))))
         return rc;
     const Block x{c->x, m, k, c->ldx}, res{c->residual, m, n, c->ld_residual}, out{c->out, m, n, c->ld_out};
     const Block pre{c->pre, m, n, c->ld_pre}, up{c->up, m, n, c->ld_up};
-    const Block wsp{static_cast<const uint32_t*>(c->workspace), 1, need / 4, 0};
+    const Block wsp{need ? static_cast<const uint32_t*>(c->workspace) : nullptr, 1, need / 4, 0};
     const bool in_place = c->residual == c->out && c->ld_residual == c->ld_out;
     if (share(wsp, x) || share(wsp, out) || share(wsp, pre) || share(wsp, up) || share(wsp, res) || share(out, x) || share(pre, x) || share(up, x) || share(out, pre) || share(out, up) || share(pre, up) ||
         (!in_place && share(out, res)) || share(pre, res))
@@ -250,8 +254,13 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     io.ld_up = c->ld_up;
     io.m = (uint32_t)m;
     io.activation = c->activation;
+    TokenPlan t;
+    if (linear_token_plan(lin->w, io.m, c->x_bits, ctx->num_sms, &t)) {
+        ZK_CUDA(launch_linear_token(lin->w, t, io, s, true));
+        ctx->launches++;
+        return ZKML_OK;
+    }
     ZK_CUDA(launch_linear(lin->w, linear_plan(lin->w, io.m, c->x_bits, ctx->num_sms), io, c->workspace, s, true));
-    ZK_CUDA(cudaGetLastError());
     ctx->launches += 2;
     return ZKML_OK;
 }

@@ -18,11 +18,7 @@
 
 #include <algorithm>
 
-#include "activation_device.cuh"
-#include "imma.cuh"
-#include "linear.cuh"
-#include "round_arith.cuh"
-#include "tcgen05.cuh"
+#include "linear_device.cuh"
 
 namespace zk {
 
@@ -33,7 +29,6 @@ namespace {
 // calls by it (64 tokens x 5120 x 13824: 58 us with 4 warps).
 constexpr uint32_t EPI_WARPS = 16, EPI_THREADS = 32 * EPI_WARPS, EPI_SUBS = EPI_WARPS / 4;
 constexpr uint32_t THREADS = 64 + EPI_THREADS;
-constexpr uint32_t KSEG = 1023;  // K tiles per 32-bit accumulation: 1023 * 128 * 2^14 < 2^31
 
 // ---------------------------------------------------------------------------
 // Weights
@@ -242,116 +237,6 @@ __device__ __forceinline__ void tile_at(const KernelArgs& a, uint32_t tile, uint
     mt = 8 * group + i - nt * high;
 }
 
-// SiLU or GELU of the M31 word v with |real| below the saturation bound, canonical.
-// Both are mag * w / (1 + e) in units of 2^-16, with mag = |v|, w = 1 for positive and e for
-// negative v, and e = exp(-a), a = |x| for SiLU and 2 |u| for GELU's inner term u
-// (1 + tanh u = 2 / (1 + exp(-2u))).  e = 2^-k exp(r), |r| <= ln(2) / 2, by the Taylor polynomial
-// of degree 9 (remainder below 2^-37), 1 / (1 + e) by one Newton step from a single-precision
-// estimate (below 2^-43): the result, below 2^21.3, is off by less than 2^-15.  Where it lies
-// within 2^-12 of a half-integer the defining binary64 form decides the rounding.  About 25
-// double-precision operations instead of the 150 and more of exp, tanh and a division.
-__device__ __forceinline__ uint32_t bent_activation(int tag, uint32_t v, uint32_t mag, bool neg) {
-    const double x = (double)mag * (1.0 / 65536.0);
-    double a = x;
-    if (tag == 2) a = 2.0 * 0.79788456080286535588 * fma(0.044715 * x * x, x, x);  // 2 sqrt(2 / pi) (x + 0.044715 x^3)
-    const int k = __double2int_rn(a * 1.44269504088896340736);  // a / ln 2
-    const double r = fma((double)k, 0.69314718055994530942, -a);
-    double e = 1.0 / 362880.0;
-    e = fma(e, r, 1.0 / 40320.0);
-    e = fma(e, r, 1.0 / 5040.0);
-    e = fma(e, r, 1.0 / 720.0);
-    e = fma(e, r, 1.0 / 120.0);
-    e = fma(e, r, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    e *= __hiloint2double((1023 - k) << 20, 0);  // k < 90
-    const double d = 1.0 + e;
-    const double q0 = (double)__fdividef(1.0f, (float)d);
-    const double q = q0 * fma(-d, q0, 2.0);
-    const double y = (double)mag * (neg ? e * q : q);
-    const double whole = floor(y), rest = y - whole;
-    if (fabs(rest - 0.5) < 1.0 / 4096.0) return red32(act_value(tag, v));
-    const uint32_t n = (uint32_t)whole + (rest >= 0.5 ? 1u : 0u);
-    return neg && n ? P - n : n;
-}
-
-// f(v), canonical.  Where SiLU and GELU equal their argument or round to zero in binary64 the
-// result is taken without evaluating them: for real x >= 37, exp(-x) < 2^-53 and 1 + exp(-x) is
-// 1; for x <= -16, |x| exp(x) 2^16 < 1/2; for |x| >= 8.5, |tanh| of GELU's inner term (above 28)
-// is 1.
-__device__ __forceinline__ uint32_t activate(int tag, uint32_t v) {
-    if (tag == 0) return v;
-    if (tag == 1) return v <= (P - 1) / 2 ? v : 0u;
-    if (tag == 5 || tag == 2) {
-        const bool neg = v > (P - 1) / 2;
-        const uint32_t mag = neg ? P - v : v;
-        const uint32_t sat = tag == 2 ? (17u << 15) : neg ? (16u << 16) : (37u << 16);
-        if (mag >= sat) return neg ? 0u : v;
-        return bent_activation(tag, v, mag, neg);
-    }
-    return red32(act_value(tag, v));
-}
-
-// Tokens handled together: their digits are 16 accumulator columns.
-template <int D>
-constexpr int GROUP = 16 / D;
-
-// sum_i 256^i acc_i mod P of one token's accumulators.
-template <int D>
-__device__ __forceinline__ uint32_t join_digits(const uint32_t (&r)[16], int t) {
-    if (D == 1) {
-        const int v = (int)r[t];
-        return red32(v < 0 ? (uint32_t)(v + 0x7fffffff) : (uint32_t)v);
-    }
-    int64_t s = 0;
-#pragma unroll
-    for (int i = D - 1; i >= 0; i--) s = s * 256 + (int)r[i * GROUP<D> + t];
-    return canon64((uint64_t)s + ((uint64_t)P << 26));  // |s| < 2^56
-}
-
-// Finishes GROUP tokens of this lane's row: z (without the bias) -> outputs.
-template <int D, bool GATED>
-__device__ __forceinline__ void finish_tokens(const KernelArgs& a, uint32_t nt, uint32_t row, uint32_t tok0,
-                                              uint32_t base, uint32_t (&z)[GROUP<D>]) {
-    const LinearIO& io = a.io;
-    constexpr int G = GROUP<D>;
-#pragma unroll
-    for (int t = 0; t < G; t++) z[t] = madd(z[t], base);
-    if (GATED) {
-        // lane l < 16: gate, lane l + 16: up of the same output; of each token pair one lane
-        // finishes the first token and the other the second
-        const bool up_lane = (row & 16) != 0;
-        const uint32_t f = nt * 64 + (row >> 5) * 16 + (row & 15);
-#pragma unroll
-        for (int t = 0; t < G; t += 2) {
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, up_lane ? z[t] : z[t + 1], 16);
-            const uint32_t g = up_lane ? got : z[t], u = up_lane ? z[t + 1] : got;
-            const uint32_t tok = tok0 + t + (up_lane ? 1 : 0);
-            if (f < a.w.n && tok < io.m) {
-                if (io.pre) io.pre[(size_t)tok * io.ld_pre + f] = g;
-                if (io.up) io.up[(size_t)tok * io.ld_up + f] = u;
-                io.out[(size_t)tok * io.ld_out + f] = mmul(activate(io.activation, g), u);
-            }
-        }
-    } else {
-        const uint32_t f = nt * LIN_ROWS + row;
-        if (f >= a.w.n) return;
-        uint32_t res[G], bad = 0;
-#pragma unroll
-        for (int t = 0; t < G; t++) res[t] = io.residual && tok0 + t < io.m ? io.residual[(size_t)(tok0 + t) * io.ld_res + f] : 0u;
-#pragma unroll
-        for (int t = 0; t < G; t++) {
-            if (tok0 + t >= io.m) continue;
-            if (io.pre) io.pre[(size_t)(tok0 + t) * io.ld_pre + f] = z[t];
-            bad |= res[t] >> 31;
-            io.out[(size_t)(tok0 + t) * io.ld_out + f] = madd(activate(io.activation, z[t]), red32(res[t]));
-        }
-        if (bad) atomicOr(io.status, LIN_BAD_VALUE);
-    }
-}
-
 // Whether `ok` holds in all epilogue threads: they go on, or give up, together.
 __device__ __forceinline__ bool all_of_epilogue(bool ok) {
     uint32_t r;
@@ -365,7 +250,6 @@ __device__ __forceinline__ bool all_of_epilogue(bool ok) {
 
 template <int D, bool GATED>
 __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constant__ KernelArgs a) {
-    grid_dependents_launch();  // the next call's digit kernel, which waits for this grid's end, may take its place
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * 16 + 5];
     __shared__ uint32_t tmem_base_s, last_s;
@@ -397,6 +281,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
+    // only now, with its tensor memory in hand: a dependent's block must not take what this grid still needs
+    grid_dependents_launch();
 
     if (warp == 0) {
         if (lane == 0) {
@@ -532,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                     for (int t = 0; t < G; t++) z[t] = madd(z[t], slot[(size_t)(t0 + t) * LIN_ROWS]);
                 }
                 if (direct) {
-                    finish_tokens<D, GATED>(a, nt, row, mt * a.tokens + t0, base, z);
+                    finish_tokens<D, GATED>(a.io, a.w.n, nt, row, mt * a.tokens + t0, base, z);
                 } else {
 #pragma unroll
                     for (int t = 0; t < G; t++) slot[(size_t)(t0 + t) * LIN_ROWS] = z[t];
@@ -580,7 +466,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                     }
 #pragma unroll
                     for (int t = 0; t < G; t++) z[t] = canon64(sum[t]);
-                    finish_tokens<D, GATED>(a, nt, row, mt * a.tokens + t0, base, z);
+                    finish_tokens<D, GATED>(a.io, a.w.n, nt, row, mt * a.tokens + t0, base, z);
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");  // last_s is read before it is written again
@@ -598,24 +484,6 @@ template <int D, bool GATED>
 cudaError_t configure_one() {
     return cudaFuncSetAttribute(linear_kernel<D, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
 }
-
-// Both kernels of a call are programmatic dependents: a block of the product kernel starts, and
-// loads weights, as soon as an SM is free, before the digits are made and before the last blocks
-// of the previous call are done; what depends on earlier work comes after grid_dependency_wait.
-struct Launch {
-    cudaLaunchAttribute attr{};
-    cudaLaunchConfig_t cfg{};
-    Launch(dim3 grid, unsigned block, size_t smem, cudaStream_t s, bool overlap) {
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cfg.gridDim = grid;
-        cfg.blockDim = dim3(block);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = s;
-        cfg.attrs = &attr;
-        cfg.numAttrs = overlap ? 1 : 0;
-    }
-};
 
 template <int D>
 cudaError_t launch_all(const KernelArgs& a, const LinearPlan& p, uint8_t* digits, cudaStream_t s, bool overlap) {

@@ -45,6 +45,24 @@ def test_linear_shapes_and_widths(m, k, n, x_bits, w_bits):
     L.same(host(lin(dev(x), x_bits=x_bits)), L.product(x, w))
 
 
+@pytest.mark.parametrize("k", [100, 512, 1000, 1024, 1500, 2047, 2600, 3100, 3600, 4096, 9000])
+@pytest.mark.parametrize("m,x_bits", [(1, 31), (3, 31), (4, 31), (5, 31), (8, 31), (9, 31), (1, 16), (8, 16), (13, 16),
+                                      (16, 16), (1, 8), (16, 8), (29, 8), (32, 8), (33, 8)])
+def test_a_few_tokens(k, m, x_bits):
+    """One to eight blocks share K; both digit widths, and the sizes around where the kernels change."""
+    n = 200
+    x, w, w2, r = ints((m, k), x_bits, 1), ints((k, n), 8, 2), ints((k, n), 8, 3), ints((m, n), 31, 4)
+    y, z, unsure = L.linear(x, w, None, 5, r)
+    got = Z.LinearM31(dev(w))(dev(x), activation="silu", residual=dev(r), keep=True, x_bits=x_bits)
+    L.same(host(got[1]), z)
+    L.same(host(got[0]), y, unsure)
+    h, g, u, unsure = L.gated(x, w, w2)
+    got = Z.GatedLinearM31(dev(w), dev(w2))(dev(x), keep=True, x_bits=x_bits)
+    L.same(host(got[1]), g)
+    L.same(host(got[2]), u)
+    L.same(host(got[0]), h, unsure)
+
+
 @pytest.mark.parametrize("act", list(TAGS))
 @pytest.mark.parametrize("bias,residual,keep", [(0, 0, 0), (1, 0, 1), (0, 1, 0), (1, 1, 1)])
 def test_linear_epilogues(act, bias, residual, keep):
