@@ -20,14 +20,17 @@ struct zkml_linear {
 namespace zk {
 namespace {
 
-// The calling thread's current device, put back when a call returns.
+// Makes `device` current and puts the calling thread's device back when a call returns.
 struct DeviceGuard {
     int prev = -1;
-    DeviceGuard() {
+    cudaError_t error;
+    explicit DeviceGuard(int device) {
         if (cudaGetDevice(&prev) != cudaSuccess) {
             cudaGetLastError();
             prev = -1;
         }
+        error = prev == device ? cudaSuccess : cudaSetDevice(device);
+        if (prev == device) prev = -1;
     }
     ~DeviceGuard() {
         if (prev >= 0) cudaSetDevice(prev);
@@ -66,6 +69,31 @@ bool share(const Block& a, const Block& b) {
     return d < lo.cols || d + hi.cols > lo.ld;
 }
 
+// The kernel of a call and its split, by sizes alone.
+struct Choice {
+    bool few;
+    TokenPlan token;
+    LinearPlan linear;
+    size_t bytes() const { return few ? 0 : linear.bytes; }
+};
+// Planning weighs dozens of splits (microseconds); a thread keeps the last ones it made.
+const Choice& choose(const PackedWeights& w, uint32_t m, int x_bits, int num_sms) {
+    struct Entry {
+        uint32_t k = 0, n = 0, planes = 0, gated = 0, m = 0;
+        int x_bits = 0, num_sms = 0;
+        Choice c;
+    };
+    static thread_local Entry kept[64];
+    Entry& e = kept[(w.k * 31 + w.n * 17 + m * 7 + w.planes + 2 * w.gated + (uint32_t)x_bits) % 64];
+    if (e.k == w.k && e.n == w.n && e.planes == w.planes && e.gated == (uint32_t)w.gated && e.m == m &&
+        e.x_bits == x_bits && e.num_sms == num_sms)
+        return e.c;
+    e.c.few = linear_token_plan(w, m, x_bits, num_sms, &e.c.token);
+    if (!e.c.few) e.c.linear = linear_plan(w, m, x_bits, num_sms);
+    e.k = w.k, e.n = w.n, e.planes = w.planes, e.gated = w.gated, e.m = m, e.x_bits = x_bits, e.num_sms = num_sms;
+    return e.c;
+}
+
 int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* biases, int parts, size_t k, size_t n,
            size_t rs, size_t cs, void* stream, zkml_linear** out) {
     if (!out) return set_error(ZKML_ERR_INVALID_ARG, "out is NULL");
@@ -78,8 +106,8 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
     if (rs > ((size_t)1 << 34) || cs > ((size_t)1 << 34) || (k - 1) * rs + (n - 1) * cs > ((size_t)1 << 36))
         return set_error(ZKML_ERR_INVALID_ARG, "weight stride too large");
-    DeviceGuard guard;
-    ZK_CUDA(cudaSetDevice(ctx->device));
+    DeviceGuard guard(ctx->device);
+    ZK_CUDA(guard.error);
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     ZK_CUDA(cudaStreamIsCapturing(s, &cap));
@@ -182,8 +210,7 @@ int zkml_linear_create_gated(zkml_ctx* ctx, const uint32_t* w_gate, const uint32
 
 int zkml_linear_destroy(zkml_linear* lin) {
     if (!lin) return ZKML_OK;
-    DeviceGuard guard;
-    cudaSetDevice(lin->ctx->device);
+    DeviceGuard guard(lin->ctx->device);
     lin->release();  // cudaFree waits for the work that reads the weights
     delete lin;
     return ZKML_OK;
@@ -196,10 +223,7 @@ int zkml_linear_workspace(const zkml_linear* lin, size_t m, int x_bits, size_t* 
     if (m == 0) return set_error(ZKML_ERR_INVALID_ARG, "empty matrix");
     if (m > (1u << 30) || m * lin->w.k > ((size_t)1 << 34) || m * lin->w.n > ((size_t)1 << 34))
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
-    TokenPlan t;
-    *out_bytes = 0;
-    if (linear_token_plan(lin->w, (uint32_t)m, x_bits, lin->ctx->num_sms, &t)) return ZKML_OK;
-    *out_bytes = linear_plan(lin->w, (uint32_t)m, x_bits, lin->ctx->num_sms).bytes;
+    *out_bytes = choose(lin->w, (uint32_t)m, x_bits, lin->ctx->num_sms).bytes();
     return ZKML_OK;
 }
 
@@ -224,9 +248,14 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     if (need && (reinterpret_cast<uintptr_t>(c->workspace) & 255))
         return set_error(ZKML_ERR_INVALID_ARG, "workspace is not aligned to 256 bytes");
     zkml_ctx* ctx = lin->ctx;
-    DeviceGuard guard;
-    ZK_CUDA(cudaSetDevice(ctx->device));
-    if ((rc = want_device_words(ctx, c->x, "x")) || (rc = want_device_words(ctx, c->out, "out")) ||
+    DeviceGuard guard(ctx->device);
+    ZK_CUDA(guard.error);
+    if (c->pointers_checked) {
+        const uintptr_t all = reinterpret_cast<uintptr_t>(c->x) | reinterpret_cast<uintptr_t>(c->out) |
+                              reinterpret_cast<uintptr_t>(c->residual) | reinterpret_cast<uintptr_t>(c->pre) |
+                              reinterpret_cast<uintptr_t>(c->up);
+        if (all & 3) return set_error(ZKML_ERR_INVALID_ARG, "an argument is not aligned to words");
+    } else if ((rc = want_device_words(ctx, c->x, "x")) || (rc = want_device_words(ctx, c->out, "out")) ||
         (need && (rc = want_device_words(ctx, c->workspace, "workspace"))) ||
         (c->residual && (rc = want_device_words(ctx, c->residual, "residual"))) ||
         (c->pre && (rc = want_device_words(ctx, c->pre, "pre"))) ||
@@ -254,21 +283,19 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     io.ld_up = c->ld_up;
     io.m = (uint32_t)m;
     io.activation = c->activation;
-    TokenPlan t;
-    if (linear_token_plan(lin->w, io.m, c->x_bits, ctx->num_sms, &t)) {
-        ZK_CUDA(launch_linear_token(lin->w, t, io, s, true));
-        ctx->launches++;
-        return ZKML_OK;
-    }
-    ZK_CUDA(launch_linear(lin->w, linear_plan(lin->w, io.m, c->x_bits, ctx->num_sms), io, c->workspace, s, true));
-    ctx->launches += 2;
+    const Choice& p = choose(lin->w, io.m, c->x_bits, ctx->num_sms);
+    if (p.few)
+        ZK_CUDA(launch_linear_token(lin->w, p.token, io, s, true));
+    else
+        ZK_CUDA(launch_linear(lin->w, p.linear, io, c->workspace, s, true));
+    ctx->launches += p.few ? 1 : 2;
     return ZKML_OK;
 }
 
 int zkml_linear_check(zkml_linear* lin, void* stream) {
     if (!lin) return set_error(ZKML_ERR_INVALID_ARG, "NULL argument");
-    DeviceGuard guard;
-    ZK_CUDA(cudaSetDevice(lin->ctx->device));
+    DeviceGuard guard(lin->ctx->device);
+    ZK_CUDA(guard.error);
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : lin->ctx->stream;
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     ZK_CUDA(cudaStreamIsCapturing(s, &cap));

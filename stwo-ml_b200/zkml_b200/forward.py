@@ -14,19 +14,17 @@ device's current torch stream.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import numpy as np
 
-from . import ACTIVATION_TAGS, InvalidArgument, _check, _fast_fn, context, lib
+from . import ACTIVATION_TAGS, InvalidArgument, _check, context, lib
 
 
-class _LinearCall(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("m", C.c_size_t), ("ldx", C.c_size_t), ("x_bits", C.c_int),
-                ("activation", C.c_int), ("residual", C.c_void_p), ("ld_residual", C.c_size_t),
-                ("out", C.c_void_p), ("ld_out", C.c_size_t), ("pre", C.c_void_p), ("ld_pre", C.c_size_t),
-                ("up", C.c_void_p), ("ld_up", C.c_size_t), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p)]
+# zkml_linear_call, field for field: x, m, ldx, x_bits, activation, residual, ld_residual, out, ld_out,
+# pre, ld_pre, up, ld_up, workspace, workspace_bytes, stream, pointers_checked
+_CALL = struct.Struct("@PNNiiPNPNPNPNPNPi4x")
 
 
 _TAGS = {None: 0, "none": 0, "relu": 1, **ACTIVATION_TAGS}
@@ -34,6 +32,9 @@ _STREAM_LEGACY = 1  # cudaStreamLegacy: torch's default stream (0) by a handle t
 
 
 def _tag(activation) -> int:
+    tag = _TAGS.get(activation)
+    if tag is not None:
+        return tag
     if isinstance(activation, str) or activation is None:
         tag = _TAGS.get(activation.lower() if isinstance(activation, str) else None)
         if tag is None:
@@ -49,7 +50,21 @@ def _is_tensor(x) -> bool:
 def _torch():
     import torch
 
+    if _i32[0] is None:
+        _i32[0] = torch.int32
     return torch
+
+
+_i32 = [None]  # torch.int32, once torch is there
+_forward_fn = []
+
+
+def _forward():
+    """zkml_linear_forward with the handle as a plain integer and the packed call as bytes."""
+    if not _forward_fn:
+        addr = C.cast(lib().zkml_linear_forward, C.c_void_p).value
+        _forward_fn.append(C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_char_p)(addr))
+    return _forward_fn[0]
 
 
 class _Weights:
@@ -61,6 +76,7 @@ class _Weights:
             device = first.device.index if _is_tensor(first) and first.is_cuda else 0
         self.device = int(device)
         self._handle = None
+        self._need = {}
         keep, ptrs, strides = [], [], []
         for w in weights:
             if len(w.shape) != 2:
@@ -127,6 +143,11 @@ class _Weights:
 
     def _rows(self, x, width, name, m=None):
         """(pointer, rows, row stride) of a matrix of words on this device; one row may be 1-D."""
+        if x.dtype is _i32[0] and x.is_cuda and x.device.index == self.device and x.dim() == 2:
+            rows, cols = x.shape
+            ld, one = x.stride()
+            if cols == width and (one == 1 or width == 1) and rows and (m is None or rows == m):
+                return x.data_ptr(), rows, ld if rows > 1 else width  # the common form, in a few attribute reads
         x = self._words(x, name)
         if not x.dim() or x.shape[-1] != width:
             raise InvalidArgument(1, f"{name} has rows of {width} words")
@@ -152,31 +173,49 @@ class _Weights:
         torch = _torch()
         if check and torch.cuda.is_current_stream_capturing():
             raise InvalidArgument(1, "the check waits for the stream; pass check=False while it is captured")
-        c = _LinearCall()
-        c.x, m, c.ldx = self._rows(x, self.k, "x")
-        c.m, c.x_bits, c.activation = m, int(x_bits), _tag(activation)
+        k, n = self.k, self.n
+        xp, m, ldx = self._rows(x, k, "x")
+        rp = ldr = op = ldo = pp = ldp = pu = ldu = ws = 0
         if residual is not None:
             if residual.dim() == 1 and m != 1:
-                residual = residual.unsqueeze(0).expand(m, self.n)  # one row for every token
-            c.residual, _, c.ld_residual = self._rows(residual, self.n, "residual", m)
-        shape = tuple(x.shape[:-1]) + (self.n,)
-        dev = x.device
-        results = []
-        for name, t, want in (("out", out, True), ("pre", pre, keep), ("up", up, keep and self._gated)):
-            if t is None and want:
-                t = torch.empty(shape, dtype=torch.int32, device=dev)
-            if t is not None:
-                p, _, ld = self._rows(t, self.n, name, m)
-                setattr(c, name, p)
-                setattr(c, "ld_" + name, ld)
-                results.append(t)
-        need = C.c_size_t(0)
-        _check(lib().zkml_linear_workspace(self._handle, m, c.x_bits, C.byref(need)))
-        if need.value:
-            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-            c.workspace, c.workspace_bytes = ws.data_ptr(), need.value
-        c.stream = self._stream()
-        _check(_fast_fn("zkml_linear_forward", 2)(self._handle.value, C.addressof(c)))
+                residual = residual.unsqueeze(0).expand(m, n)  # one row for every token
+            rp, _, ldr = self._rows(residual, n, "residual", m)
+        if out is None or (keep and (pre is None or (up is None and self._gated))):
+            shape = (*x.shape[:-1], n)
+        if out is None:
+            out = torch.empty(shape, dtype=torch.int32, device=x.device)
+            op, ldo = out.data_ptr(), n
+        else:
+            op, _, ldo = self._rows(out, n, "out", m)
+        results = [out]
+        if pre is not None:
+            pp, _, ldp = self._rows(pre, n, "pre", m)
+        elif keep:
+            pre = torch.empty(shape, dtype=torch.int32, device=x.device)
+            pp, ldp = pre.data_ptr(), n
+        if pre is not None:
+            results.append(pre)
+        if up is not None:
+            pu, _, ldu = self._rows(up, n, "up", m)
+        elif keep and self._gated:
+            up = torch.empty(shape, dtype=torch.int32, device=x.device)
+            pu, ldu = up.data_ptr(), n
+        if up is not None:
+            results.append(up)
+        need = self._need.get((m, x_bits))
+        if need is None:
+            size = C.c_size_t(0)
+            _check(lib().zkml_linear_workspace(self._handle, m, int(x_bits), C.byref(size)))
+            if len(self._need) > 1000:
+                self._need.clear()
+            need = self._need[(m, x_bits)] = size.value
+        if need:
+            keep_ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+            ws = keep_ws.data_ptr()
+        stream = torch._C._cuda_getCurrentRawStream(self.device) or _STREAM_LEGACY
+        call = _CALL.pack(xp, m, ldx, int(x_bits), _tag(activation), rp, ldr, op, ldo, pp, ldp, pu, ldu, ws, need, stream,
+                          1)
+        _check(_forward()(self._handle.value, call))
         if check:
             self.check()
         return results

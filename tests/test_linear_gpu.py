@@ -1,4 +1,6 @@
 """Forward operators on the GPU against their plain 64-bit forms: every output word is equal."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -304,30 +306,38 @@ def test_refused_calls():
         lin(x)
 
 
+class LinearCall(C.Structure):
+    """zkml_linear_call."""
+    _fields_ = [("x", C.c_void_p), ("m", C.c_size_t), ("ldx", C.c_size_t), ("x_bits", C.c_int), ("activation", C.c_int),
+                ("residual", C.c_void_p), ("ld_residual", C.c_size_t), ("out", C.c_void_p), ("ld_out", C.c_size_t),
+                ("pre", C.c_void_p), ("ld_pre", C.c_size_t), ("up", C.c_void_p), ("ld_up", C.c_size_t),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p),
+                ("pointers_checked", C.c_int)]
+
+
 def _c_call(lin, **kw):
-    from zkml_b200.forward import _LinearCall
-    import ctypes as C
-    c = _LinearCall()
+    c = LinearCall()
     for key, v in kw.items():
         setattr(c, key, v.data_ptr() if hasattr(v, "data_ptr") else v)
     return Z.lib().zkml_linear_forward(lin._handle, C.addressof(c))
 
 
 def test_refused_at_the_c_boundary():
-    import ctypes as C
     w = ints((40, 30), 8, 2)
     lin, gat = Z.LinearM31(dev(w)), Z.GatedLinearM31(dev(w), dev(w))
-    x = torch.zeros(4, 40, dtype=torch.int32, device="cuda")
-    o, q = (torch.zeros(4, 30, dtype=torch.int32, device="cuda") for _ in range(2))
+    x = torch.zeros(40, 40, dtype=torch.int32, device="cuda")
+    o, q = (torch.zeros(40, 30, dtype=torch.int32, device="cuda") for _ in range(2))
     need = C.c_size_t()
-    assert Z.lib().zkml_linear_workspace(lin._handle, 4, 31, C.byref(need)) == 0
+    assert Z.lib().zkml_linear_workspace(lin._handle, 40, 31, C.byref(need)) == 0
     ws = torch.empty(max(need.value, 1), dtype=torch.uint8, device="cuda")
-    good = dict(x=x, m=4, ldx=40, x_bits=31, out=o, ld_out=30, workspace=ws, workspace_bytes=need.value, stream=1)
+    good = dict(x=x, m=40, ldx=40, x_bits=31, out=o, ld_out=30, workspace=ws, workspace_bytes=need.value, stream=1)
     assert _c_call(lin, **good) == 0
     for change in (dict(x=None), dict(out=None), dict(m=0), dict(m=1 << 40), dict(ld_out=29), dict(x_bits=32),
                    dict(activation=6), dict(x=x.data_ptr() + 2), dict(x=x.cpu()), dict(out=o.cpu()), dict(up=q, ld_up=30),
                    dict(pre=q, ld_pre=29), dict(ldx=1 << 40)):
         assert _c_call(lin, **{**good, **change}) == 1, change
+    assert _c_call(lin, **good, pointers_checked=1) == 0
+    assert _c_call(lin, **{**good, "x": x.data_ptr() + 2}, pointers_checked=1) == 1
     if need.value:
         assert _c_call(lin, **{**good, "workspace": None}) == 1
         assert _c_call(lin, **{**good, "workspace_bytes": need.value - 1}) == 1
