@@ -24,7 +24,7 @@ __device__ __forceinline__ uint32_t act_from_real(double r) {
     return (uint32_t)((uint64_t)P - neg);
 }
 // v canonical.  A negative real that rounds to zero comes out as P, as in the reference.
-static __device__ uint32_t act_value(int tag, uint32_t v) {
+static __device__ __noinline__ uint32_t act_value(int tag, uint32_t v) {
     switch (tag) {
         case 1:  // ReLU
             return v <= (P - 1) / 2 ? v : 0u;

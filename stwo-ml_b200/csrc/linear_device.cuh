@@ -20,7 +20,8 @@ constexpr uint32_t KSEG = 1023;  // K tiles per 32-bit accumulation: 1023 * 128 
 // estimate (below 2^-43): the result, below 2^21.3, is off by less than 2^-15.  Where it lies
 // within 2^-12 of a half-integer the defining binary64 form decides the rounding.  About 25
 // double-precision operations instead of the 150 and more of exp, tanh and a division.
-__device__ __forceinline__ uint32_t bent_activation(int tag, uint32_t v, uint32_t mag, bool neg) {
+// Out of line: copies at every call site made the kernels miss the instruction cache.
+static __device__ __noinline__ uint32_t bent_activation(int tag, uint32_t v, uint32_t mag, bool neg) {
     const double x = (double)mag * (1.0 / 65536.0);
     double a = x;
     if (tag == 2) a = 2.0 * 0.79788456080286535588 * fma(0.044715 * x * x, x, x);  // 2 sqrt(2 / pi) (x + 0.044715 x^3)
