@@ -12,6 +12,31 @@ namespace zk {
 
 constexpr uint32_t KSEG = 1023;  // K tiles per 32-bit accumulation: 1023 * 128 * 2^14 < 2^31
 
+// The four balanced byte digits of v (|v| < 2^31 - 2^23), byte i holding the digit of 256^i in
+// [-128, 127]: adding 128 to every digit makes them the plain base-256 digits of v + 0x80808080.
+__device__ __forceinline__ uint32_t balanced_digits(int v) { return ((uint32_t)v + 0x80808080u) ^ 0x80808080u; }
+
+// The words of four activations -> D words, word b holding the four digits of 256^b (D as in
+// linear_kernels.cu); sets the status bits that apply.
+template <int D>
+__device__ __forceinline__ void activation_digits(const uint4& x, uint32_t (&d)[D], uint32_t& bad) {
+    constexpr int OFFSET = D > 1 ? 128 : 0;
+    const int v[4] = {m31_signed(x.x) - OFFSET, m31_signed(x.y) - OFFSET, m31_signed(x.z) - OFFSET,
+                      m31_signed(x.w) - OFFSET};
+    if ((x.x | x.y | x.z | x.w) >> 31) bad |= LIN_BAD_VALUE;
+    if (D < 4) {
+        constexpr uint32_t LOW = D == 1 ? 128u : 32896u, SPAN = D == 1 ? 256u : 65536u;  // D digits: [-LOW, SPAN - LOW)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if ((uint32_t)v[i] + LOW >= SPAN) bad |= LIN_BAD_RANGE;
+    }
+    uint32_t p[4];
+    byte_planes(make_uint4(balanced_digits(v[0]), balanced_digits(v[1]), balanced_digits(v[2]), balanced_digits(v[3])),
+                p[0], p[1], p[2], p[3]);
+#pragma unroll
+    for (int b = 0; b < D; b++) d[b] = p[b];
+}
+
 // SiLU or GELU of the M31 word v with |real| below the saturation bound, canonical.
 // Both are mag * w / (1 + e) in units of 2^-16, with mag = |v|, w = 1 for positive and e for
 // negative v, and e = exp(-a), a = |x| for SiLU and 2 |u| for GELU's inner term u

@@ -61,18 +61,19 @@ __global__ void __launch_bounds__(256) linear_pack_kernel(const uint32_t* __rest
         unsigned long long sum = 0;
         if (f < p.n) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                uint32_t v = k0 + i < p.k ? __ldg(src + (size_t)(k0 + i) * rs + (size_t)f * cs) : 0u;
-                bad |= v >> 31;
-                int q = m31_signed(v);
-                sum += (unsigned long long)(q < 0 ? q + (int)P : q);
-                need = max(need, planes_needed(q));
+            for (int i = 0; i < 4; i++) {
+                uint32_t q[4];
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const int g = sdigit(q);
-                    d[b][i >> 2] |= (uint32_t)(uint8_t)g << (8 * (i & 3));
-                    q = (q - g) >> 8;
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t at = k0 + 4 * i + j;
+                    const uint32_t v = at < p.k ? __ldg(src + (size_t)at * rs + (size_t)f * cs) : 0u;
+                    bad |= v >> 31;
+                    const int s = m31_signed(v);
+                    sum += (unsigned long long)(s < 0 ? s + (int)P : s);
+                    need = max(need, planes_needed(s));
+                    q[j] = balanced_digits(s);
                 }
+                byte_planes(make_uint4(q[0], q[1], q[2], q[3]), d[0][i], d[1][i], d[2][i], d[3][i]);
             }
         }
         const size_t plane = (size_t)p.n_tiles * p.k_tiles * LIN_TILE_BYTES;
@@ -123,30 +124,23 @@ __global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* __re
     const uint32_t t = blockIdx.y * 32 + threadIdx.x / 8, c = threadIdx.x % 8;
     if (t < tokens) {
         const uint32_t row = mt * tokens + t, k0 = kt * LIN_KB + 16 * c;
-        uint32_t v[16];
+        uint4 v[4];
         const uint32_t* src = x + (size_t)row * ldx + k0;
         if (row < m && vec && k0 + 16 <= k) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint4 q = __ldg(reinterpret_cast<const uint4*>(src) + i);
-                v[4 * i] = q.x, v[4 * i + 1] = q.y, v[4 * i + 2] = q.z, v[4 * i + 3] = q.w;
-            }
+            for (int i = 0; i < 4; i++) v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
         } else {
+            const auto at = [&](uint32_t i) { return row < m && k0 + i < k ? __ldg(src + i) : 0u; };
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = (row < m && k0 + i < k) ? __ldg(src + i) : 0u;
+            for (uint32_t i = 0; i < 4; i++) v[i] = make_uint4(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));
         }
-        uint32_t d[D][4] = {};
+        uint32_t d[D][4];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            if (v[i] >> 31) bad |= LIN_BAD_VALUE;
-            int q = m31_signed(v[i]) - (D > 1 ? 128 : 0);
+        for (int i = 0; i < 4; i++) {
+            uint32_t q[D];
+            activation_digits<D>(v[i], q, bad);
 #pragma unroll
-            for (int b = 0; b < D; b++) {
-                const int g = sdigit(q);
-                d[b][i >> 2] |= (uint32_t)(uint8_t)g << (8 * (i & 3));
-                q = (q - g) >> 8;
-            }
-            if (D < 4 && q != 0) bad |= LIN_BAD_RANGE;
+            for (int b = 0; b < D; b++) d[b][i] = q[b];
         }
 #pragma unroll
         for (int b = 0; b < D; b++) {

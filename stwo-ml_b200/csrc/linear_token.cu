@@ -169,20 +169,8 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
 #pragma unroll
             for (uint32_t t = 0; t < 4; t++) {
                 if (t0 + t >= a.io.m) continue;
-                const uint32_t e[4] = {v[t].x, v[t].y, v[t].z, v[t].w};
-                uint32_t d[D] = {};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if (e[i] >> 31) bad |= LIN_BAD_VALUE;
-                    int q = m31_signed(e[i]) - (D > 1 ? 128 : 0);
-#pragma unroll
-                    for (int b = 0; b < D; b++) {
-                        const int g = sdigit(q);
-                        d[b] |= (uint32_t)(uint8_t)g << (8 * i);
-                        q = (q - g) >> 8;
-                    }
-                    if (D < 4 && q != 0) bad |= LIN_BAD_RANGE;
-                }
+                uint32_t d[D];
+                activation_digits<D>(v[t], d, bad);
 #pragma unroll
                 for (int b = 0; b < D; b++) {
                     const uint32_t r = b * a.tokens + t0 + t;
