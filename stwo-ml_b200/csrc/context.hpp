@@ -107,6 +107,14 @@ struct OpeningScratch {
         for (DevBuf* b : all) b->release();
     }
 };
+// Device scratch of the forward pass's products with weights used once (grown on demand).
+struct LinearScratch {
+    DevBuf tiles, sums, base, status, workspace;
+    void release() {
+        DevBuf* all[] = {&tiles, &sums, &base, &status, &workspace};
+        for (DevBuf* b : all) b->release();
+    }
+};
 }  // namespace zk
 
 struct zkml_ctx {
@@ -135,6 +143,7 @@ struct zkml_ctx {
     zk::DevBuf rsqrt_table;         // RMSNorm rsqrt table (device copy)
     zk::LogupScratch lu;
     zk::OpeningScratch op;
+    zk::LinearScratch lin;
     zk::DevBuf gather_dev;          // gathered shards of the sharded product sumcheck
     zk::DevBuf mesh_stage;          // this rank's contribution to a mesh gather
     uint8_t* h_stage = nullptr;     // pinned host staging for the sharded gather

@@ -4,7 +4,7 @@
 // Sequential weight-binding mode, serialized by serialize_gkr_model_proof
 // (cairo_serde.rs:1307-1772) or as the verify_model_gkr calldata (starknet.rs:3143-3345).
 //
-// Forward pass on the GPU (tensor-pipe M31 GEMM, ReLU), then the transcript: depth, input
+// Forward pass on the GPU (each Linear layer with the activation or sum behind it), then the transcript: depth, input
 // shape, optional policy commitment, the output claim at a drawn point, the walk from the
 // output layer to the input (matmul layers through zkml_reduce_matmul_layer_gkr, ReLU
 // layers through the algebraic reduction, RMSNorm layers through the RMSNorm reduction, Add
@@ -27,6 +27,7 @@
 #include "channel.hpp"
 #include "context.hpp"
 #include "gkr.cuh"
+#include "linear.cuh"
 #include "logup.cuh"
 #include "mesh.hpp"
 #include "opening.hpp"
@@ -195,12 +196,24 @@ static int prove_chain(zkml_ctx* ctx, const uint64_t* model_id, const uint32_t* 
         ctx->launches++;
     }
     auto in_of = [&](size_t l) { return outs[src[l] + 1].as<uint32_t>(); };
+    if ((rc = linear_once_begin(ctx))) return rc;
     for (size_t l = 0; l < n_layers; l++) {
         const size_t w = width[src[l] + 1];
         const int t = layers[l].type;
         if (t == ZKML_LAYER_LINEAR) {
-            if ((rc = zkml_matmul_m31(ctx, in_of(l), m, w, layers[l].weight, width[l + 1], outs[l + 1].as<uint32_t>())))
-                return rc;
+            // with the activation or the sum that takes this layer's output alone, in one call
+            const int nt = l + 1 < n_layers && src[l + 1] == (long long)l ? layers[l + 1].type : -1;
+            const bool act = nt == ZKML_LAYER_RELU || nt == ZKML_LAYER_ACTIVATION;
+            const bool add = nt == ZKML_LAYER_ADD && layers[l + 1].lhs != (long long)l;
+            const int tag = nt == ZKML_LAYER_RELU ? 1 : nt == ZKML_LAYER_ACTIVATION ? (int)layers[l + 1].n : 0;
+            uint32_t* own = outs[l + 1].as<uint32_t>();
+            rc = linear_once(ctx, in_of(l), m, w, layers[l].weight, width[l + 1], tag,
+                             add ? outs[layers[l + 1].lhs + 1].as<uint32_t>() : nullptr, act || add ? own : nullptr,
+                             act || add ? outs[l + 2].as<uint32_t>() : own);
+            if (!rc && (act || add)) l++;
+            // no room for the weights' layout: the product that reads them in place
+            if (rc == ZKML_ERR_OOM) rc = zkml_matmul_m31(ctx, in_of(l), m, w, layers[l].weight, width[l + 1], own);
+            if (rc) return rc;
         } else if (t == ZKML_LAYER_RMSNORM) {
             if (!ctx->rsqrt_table.ptr) {
                 if ((rc = ctx->rsqrt_table.ensure(4u << 16))) return rc;
@@ -233,6 +246,7 @@ static int prove_chain(zkml_ctx* ctx, const uint64_t* model_id, const uint32_t* 
         }
     }
     ZK_CUDA(cudaGetLastError());
+    if ((rc = linear_once_end(ctx))) return rc;
 
     // io commitment (aggregation.rs:235-254) of the model input and output: a sequential
     // Poseidon sponge over every element (one permutation per two elements), known as soon as

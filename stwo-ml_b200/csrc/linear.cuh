@@ -4,6 +4,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+struct zkml_ctx;
+
 namespace zk {
 
 // Bits of a handle's status word.
@@ -46,6 +48,7 @@ struct LinearIO {
     size_t ldx, ld_res, ld_out, ld_pre, ld_up;
     uint32_t m;
     int activation;
+    bool as_reference = false;  // an activation that rounds a negative value to zero gives the word P, not 0
 };
 
 // How a call is split: fixed by the sizes alone.
@@ -77,5 +80,15 @@ cudaError_t linear_configure();  // per device, before the first launch
 // that work still runs.
 cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, void* workspace,
                           cudaStream_t s, bool overlap);
+
+// One product with weights that are used once (the chain prover's forward pass): lays w (k x n,
+// row major, host or device memory) out in the context's scratch and runs the call on its stream.
+// x, residual, pre and out are dense device matrices; pre may be NULL.  ZKML_ERR_OOM leaves
+// nothing done.  A run of calls is opened by _begin and closed by _end, which waits for the stream
+// and reports what the calls met.
+int linear_once_begin(::zkml_ctx* ctx);
+int linear_once_end(::zkml_ctx* ctx);
+int linear_once(::zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint32_t* w, size_t n, int activation,
+                const uint32_t* residual, uint32_t* pre, uint32_t* out);
 
 }  // namespace zk

@@ -94,6 +94,60 @@ const Choice& choose(const PackedWeights& w, uint32_t m, int x_bits, int num_sms
     return e.c;
 }
 
+int status_error(uint32_t st) {
+    if (st & LIN_BAD_VALUE)
+        return set_error(ZKML_ERR_INVALID_ARG, "linear: input value >= 2^31 is not an M31 element");
+    if (st & LIN_TIMEOUT) return set_error(ZKML_ERR_TIMEOUT, "linear: a wait inside the product kernel ran out");
+    if (st) return set_error(ZKML_ERR_INVALID_ARG, "linear: an activation does not fit the declared x_bits");
+    return ZKML_OK;
+}
+
+void set_shape(PackedWeights& w, size_t k, size_t n, bool gated) {
+    w.k = (uint32_t)k;
+    w.n = (uint32_t)n;
+    w.gated = gated;
+    w.k_tiles = (uint32_t)((k + LIN_KB - 1) / LIN_KB);
+    w.n_tiles = (uint32_t)((n + lin_outputs_per_tile(gated) - 1) / lin_outputs_per_tile(gated));
+}
+
+// Lays out weights of shape w from device memory (src: the weights, then the biases) and waits;
+// *bad: a word >= 2^31 was among them.  Signed bytes in most models: one plane is packed, and again
+// with more where a value needs them.
+int lay_out(zkml_ctx* ctx, PackedWeights& w, const uint32_t* const src[4], size_t rs, size_t cs, DevBuf& tiles,
+            DevBuf& sums, DevBuf& base, DevBuf& status, cudaStream_t s, uint32_t* bad) {
+    const size_t slots = (size_t)w.n_tiles * LIN_ROWS, plane = (size_t)w.n_tiles * w.k_tiles * LIN_TILE_BYTES;
+    int rc;
+    ZK_CUDA(linear_configure());
+    ZK_CUDA(linear_token_configure());
+    if ((rc = status.ensure(16)) || (rc = base.ensure(2 * slots * 4)) || (rc = sums.ensure(slots * 8))) return rc;
+    uint32_t st[2] = {0, 1};
+    for (w.planes = 1;; w.planes = st[1]) {
+        if ((rc = tiles.ensure(plane * w.planes))) return rc;
+        ZK_CUDA(cudaMemsetAsync(status.ptr, 0, 16, s));
+        ZK_CUDA(cudaMemsetAsync(sums.ptr, 0, slots * 8, s));
+        launch_linear_pack(src[0], src[1], rs, cs, w, tiles.as<uint8_t>(), sums.as<unsigned long long>(),
+                           status.as<uint32_t>(), s);
+        ZK_CUDA(cudaGetLastError());
+        launch_linear_base(sums.as<unsigned long long>(), src[2], src[3], w, base.as<uint32_t>(),
+                           status.as<uint32_t>(), s);
+        ZK_CUDA(cudaGetLastError());
+        ctx->launches += 2;
+        ZK_CUDA(cudaMemcpyAsync(st, status.ptr, 8, cudaMemcpyDeviceToHost, s));
+        ZK_CUDA(cudaStreamSynchronize(s));
+        if (st[0] || st[1] <= w.planes) break;
+    }
+    *bad = st[0];
+    w.tiles = tiles.as<uint8_t>();
+    w.base = base.as<uint32_t>();
+    return ZKML_OK;
+}
+
+cudaError_t launch_choice(const Choice& p, const PackedWeights& w, const LinearIO& io, void* workspace, cudaStream_t s,
+                          bool overlap) {
+    return p.few ? launch_linear_token(w, p.token, io, s, overlap)
+                 : launch_linear(w, p.linear, io, workspace, s, overlap);
+}
+
 int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* biases, int parts, size_t k, size_t n,
            size_t rs, size_t cs, void* stream, zkml_linear** out) {
     if (!out) return set_error(ZKML_ERR_INVALID_ARG, "out is NULL");
@@ -113,8 +167,6 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     ZK_CUDA(cudaStreamIsCapturing(s, &cap));
     if (cap != cudaStreamCaptureStatusNone)
         return set_error(ZKML_ERR_INVALID_ARG, "weights cannot be laid out while the stream is captured");
-    ZK_CUDA(linear_configure());
-    ZK_CUDA(linear_token_configure());
     zkml_linear* lin = new zkml_linear();
     struct Drop {
         zkml_linear*& l;
@@ -130,12 +182,7 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     } drop{lin, {}, {}};
     lin->ctx = ctx;
     PackedWeights& w = lin->w;
-    w.k = (uint32_t)k;
-    w.n = (uint32_t)n;
-    w.gated = parts == 2;
-    w.k_tiles = (uint32_t)((k + LIN_KB - 1) / LIN_KB);
-    w.n_tiles = (uint32_t)((n + lin_outputs_per_tile(w.gated) - 1) / lin_outputs_per_tile(w.gated));
-    const size_t slots = (size_t)w.n_tiles * LIN_ROWS, plane = (size_t)w.n_tiles * w.k_tiles * LIN_TILE_BYTES;
+    set_shape(w, k, n, parts == 2);
     const uint32_t* dev[4] = {};  // weights, then biases
     int rc;
     for (int g = 0; g < 2 * parts; g++) {
@@ -162,34 +209,65 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
         ctx->h2d_bytes += bytes;
         *to = drop.stage[g].as<uint32_t>();
     }
-    if ((rc = lin->status.ensure(16)) || (rc = lin->base.ensure(2 * slots * 4)) || (rc = drop.sums.ensure(slots * 8)))
-        return rc;
-    // signed bytes in most models: pack one plane, and again with more where a value needs them
-    uint32_t st[2] = {0, 1};
-    for (w.planes = 1;; w.planes = st[1]) {
-        if ((rc = lin->tiles.ensure(plane * w.planes))) return rc;
-        ZK_CUDA(cudaMemsetAsync(lin->status.ptr, 0, 16, s));
-        ZK_CUDA(cudaMemsetAsync(drop.sums.ptr, 0, slots * 8, s));
-        launch_linear_pack(dev[0], dev[1], rs, cs, w, lin->tiles.as<uint8_t>(), drop.sums.as<unsigned long long>(),
-                           lin->status.as<uint32_t>(), s);
-        ZK_CUDA(cudaGetLastError());
-        launch_linear_base(drop.sums.as<unsigned long long>(), dev[2], dev[3], w, lin->base.as<uint32_t>(),
-                           lin->status.as<uint32_t>(), s);
-        ZK_CUDA(cudaGetLastError());
-        ctx->launches += 2;
-        ZK_CUDA(cudaMemcpyAsync(st, lin->status.ptr, 8, cudaMemcpyDeviceToHost, s));
-        ZK_CUDA(cudaStreamSynchronize(s));
-        if (st[0]) return set_error(ZKML_ERR_INVALID_ARG, "linear: weight or bias value >= 2^31 is not an M31 element");
-        if (st[1] <= w.planes) break;
-    }
-    w.tiles = lin->tiles.as<uint8_t>();
-    w.base = lin->base.as<uint32_t>();
+    uint32_t bad = 0;
+    if ((rc = lay_out(ctx, w, dev, rs, cs, lin->tiles, drop.sums, lin->base, lin->status, s, &bad))) return rc;
+    if (bad) return set_error(ZKML_ERR_INVALID_ARG, "linear: weight or bias value >= 2^31 is not an M31 element");
     *out = lin;
     lin = nullptr;
     return ZKML_OK;
 }
 
 }  // namespace
+
+// Words 4 and up of the scratch status collect what the calls meet; lay_out uses those before.
+int linear_once_begin(zkml_ctx* ctx) {
+    const int rc = ctx->lin.status.ensure(256);
+    if (rc) return rc;
+    ZK_CUDA(cudaMemsetAsync(ctx->lin.status.ptr, 0, 256, ctx->stream));
+    return ZKML_OK;
+}
+
+int linear_once_end(zkml_ctx* ctx) {
+    uint32_t st = 0;
+    ZK_CUDA(cudaMemcpyAsync(&st, ctx->lin.status.as<uint32_t>() + 4, 4, cudaMemcpyDeviceToHost, ctx->stream));
+    ZK_CUDA(cudaStreamSynchronize(ctx->stream));
+    return status_error(st);
+}
+
+int linear_once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint32_t* w, size_t n, int activation,
+                const uint32_t* residual, uint32_t* pre, uint32_t* out) {
+    if (m > (1u << 30) || k > (1u << 30) || n > (1u << 30) || m * k > ((size_t)1 << 34) || k * n > ((size_t)1 << 34) ||
+        m * n > ((size_t)1 << 34))
+        return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
+    LinearScratch& b = ctx->lin;
+    cudaStream_t s = ctx->stream;
+    const void* dev = nullptr;
+    PackedWeights p;
+    set_shape(p, k, n, false);
+    uint32_t bad = 0;
+    int rc = device_view(ctx, w, k * n * 4, ctx->b_in, &dev);
+    const uint32_t* src[4] = {static_cast<const uint32_t*>(dev), nullptr, nullptr, nullptr};
+    if (!rc) rc = lay_out(ctx, p, src, n, 1, b.tiles, b.sums, b.base, b.status, s, &bad);
+    if (rc) return rc;
+    if (bad) return set_error(ZKML_ERR_INVALID_ARG, "matmul_m31: input value >= 2^31 is not an M31 element");
+    const Choice& c = choose(p, (uint32_t)m, 31, ctx->num_sms);
+    if ((rc = b.workspace.ensure(c.bytes()))) return rc;
+    LinearIO io{};
+    io.x = x;
+    io.residual = residual;
+    io.out = out;
+    io.pre = pre;
+    io.status = b.status.as<uint32_t>() + 4;
+    io.ldx = k;
+    io.ld_res = io.ld_out = io.ld_pre = n;
+    io.m = (uint32_t)m;
+    io.activation = activation;
+    io.as_reference = true;
+    ZK_CUDA(launch_choice(c, p, io, b.workspace.ptr, s, false));
+    ctx->launches += c.few ? 1 : 2;
+    return ZKML_OK;
+}
+
 }  // namespace zk
 
 using namespace zk;
@@ -284,10 +362,7 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     io.m = (uint32_t)m;
     io.activation = c->activation;
     const Choice& p = choose(lin->w, io.m, c->x_bits, ctx->num_sms);
-    if (p.few)
-        ZK_CUDA(launch_linear_token(lin->w, p.token, io, s, true));
-    else
-        ZK_CUDA(launch_linear(lin->w, p.linear, io, c->workspace, s, true));
+    ZK_CUDA(launch_choice(p, lin->w, io, c->workspace, s, true));
     ctx->launches += p.few ? 1 : 2;
     return ZKML_OK;
 }
@@ -304,12 +379,8 @@ int zkml_linear_check(zkml_linear* lin, void* stream) {
     uint32_t st = 0;
     ZK_CUDA(cudaMemcpyAsync(&st, lin->status.ptr, 4, cudaMemcpyDeviceToHost, s));
     ZK_CUDA(cudaStreamSynchronize(s));
-    if (!st) return ZKML_OK;
-    ZK_CUDA(cudaMemsetAsync(lin->status.ptr, 0, 4, s));
-    if (st & LIN_BAD_VALUE)
-        return set_error(ZKML_ERR_INVALID_ARG, "linear: input value >= 2^31 is not an M31 element");
-    if (st & LIN_TIMEOUT) return set_error(ZKML_ERR_TIMEOUT, "linear: a wait inside the product kernel ran out");
-    return set_error(ZKML_ERR_INVALID_ARG, "linear: an activation does not fit the declared x_bits");
+    if (st) ZK_CUDA(cudaMemsetAsync(lin->status.ptr, 0, 4, s));
+    return status_error(st);
 }
 
 }  // extern "C"

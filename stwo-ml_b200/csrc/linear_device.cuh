@@ -107,6 +107,12 @@ __device__ __forceinline__ uint32_t join_digits(const uint32_t (&r)[16], int t) 
     return canon64((uint64_t)s + ((uint64_t)P << 26));  // |s| < 2^56
 }
 
+// f(v) as an output word: canonical, or as the reference's forward pass leaves it (LinearIO::as_reference).
+__device__ __forceinline__ uint32_t activated(const LinearIO& io, uint32_t v) {
+    if (io.as_reference && io.activation) return act_value(io.activation, v);
+    return activate(io.activation, v);
+}
+
 // Finishes GROUP tokens of this lane's row: z (without the bias) -> outputs.
 template <int D, bool GATED>
 __device__ __forceinline__ void finish_tokens(const LinearIO& io, uint32_t n, uint32_t nt, uint32_t row, uint32_t tok0,
@@ -127,7 +133,7 @@ __device__ __forceinline__ void finish_tokens(const LinearIO& io, uint32_t n, ui
             if (f < n && tok < io.m) {
                 if (io.pre) io.pre[(size_t)tok * io.ld_pre + f] = g;
                 if (io.up) io.up[(size_t)tok * io.ld_up + f] = u;
-                io.out[(size_t)tok * io.ld_out + f] = mmul(activate(io.activation, g), u);
+                io.out[(size_t)tok * io.ld_out + f] = mmul(activated(io, g), u);
             }
         }
     } else {
@@ -141,7 +147,8 @@ __device__ __forceinline__ void finish_tokens(const LinearIO& io, uint32_t n, ui
             if (tok0 + t >= io.m) continue;
             if (io.pre) io.pre[(size_t)(tok0 + t) * io.ld_pre + f] = z[t];
             bad |= res[t] >> 31;
-            io.out[(size_t)(tok0 + t) * io.ld_out + f] = madd(activate(io.activation, z[t]), red32(res[t]));
+            const uint32_t y = activated(io, z[t]);
+            io.out[(size_t)(tok0 + t) * io.ld_out + f] = io.residual ? madd(y, red32(res[t])) : y;
         }
         if (bad) atomicOr(io.status, LIN_BAD_VALUE);
     }

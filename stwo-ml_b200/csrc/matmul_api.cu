@@ -850,6 +850,7 @@ int zkml_ctx_destroy(zkml_ctx* ctx) {
     ctx->rsqrt_table.release();
     ctx->lu.release();
     ctx->op.release();
+    ctx->lin.release();
     ctx->gather_dev.release();
     ctx->mesh_stage.release();
     if (ctx->h_stage) cudaFreeHost(ctx->h_stage);
