@@ -109,9 +109,11 @@ struct OpeningScratch {
 };
 // Device scratch of the forward pass's products with weights used once (grown on demand).
 struct LinearScratch {
-    DevBuf tiles, sums, base, status, workspace;
+    DevBuf tiles, small;  // as a zkml_linear's
+    DevBuf met;           // what the calls of a run met (status bits)
+    DevBuf workspace;
     void release() {
-        DevBuf* all[] = {&tiles, &sums, &base, &status, &workspace};
+        DevBuf* all[] = {&tiles, &small, &met, &workspace};
         for (DevBuf* b : all) b->release();
     }
 };

@@ -9,11 +9,11 @@
 struct zkml_linear {
     zkml_ctx* ctx = nullptr;
     zk::PackedWeights w;
-    zk::DevBuf tiles, base, status;
+    zk::DevBuf tiles;
+    zk::DevBuf small;  // status words, column sums, per-row constants
     void release() {
         tiles.release();
-        base.release();
-        status.release();
+        small.release();
     }
 };
 
@@ -102,6 +102,8 @@ int status_error(uint32_t st) {
     return ZKML_OK;
 }
 
+constexpr size_t STATUS_BYTES = 256;
+
 void set_shape(PackedWeights& w, size_t k, size_t n, bool gated) {
     w.k = (uint32_t)k;
     w.n = (uint32_t)n;
@@ -114,31 +116,31 @@ void set_shape(PackedWeights& w, size_t k, size_t n, bool gated) {
 // *bad: a word >= 2^31 was among them.  Signed bytes in most models: one plane is packed, and again
 // with more where a value needs them.
 int lay_out(zkml_ctx* ctx, PackedWeights& w, const uint32_t* const src[4], size_t rs, size_t cs, DevBuf& tiles,
-            DevBuf& sums, DevBuf& base, DevBuf& status, cudaStream_t s, uint32_t* bad) {
+            DevBuf& small, cudaStream_t s, uint32_t* bad) {
     const size_t slots = (size_t)w.n_tiles * LIN_ROWS, plane = (size_t)w.n_tiles * w.k_tiles * LIN_TILE_BYTES;
     int rc;
     ZK_CUDA(linear_configure());
     ZK_CUDA(linear_token_configure());
-    if ((rc = status.ensure(16)) || (rc = base.ensure(2 * slots * 4)) || (rc = sums.ensure(slots * 8))) return rc;
+    if ((rc = small.ensure(STATUS_BYTES + slots * 16))) return rc;
+    uint32_t* const status = small.as<uint32_t>();
+    unsigned long long* const sums = reinterpret_cast<unsigned long long*>(small.as<uint8_t>() + STATUS_BYTES);
+    uint32_t* const base = reinterpret_cast<uint32_t*>(sums + slots);
     uint32_t st[2] = {0, 1};
     for (w.planes = 1;; w.planes = st[1]) {
         if ((rc = tiles.ensure(plane * w.planes))) return rc;
-        ZK_CUDA(cudaMemsetAsync(status.ptr, 0, 16, s));
-        ZK_CUDA(cudaMemsetAsync(sums.ptr, 0, slots * 8, s));
-        launch_linear_pack(src[0], src[1], rs, cs, w, tiles.as<uint8_t>(), sums.as<unsigned long long>(),
-                           status.as<uint32_t>(), s);
+        ZK_CUDA(cudaMemsetAsync(status, 0, STATUS_BYTES + slots * 8, s));
+        launch_linear_pack(src[0], src[1], rs, cs, w, tiles.as<uint8_t>(), sums, status, s);
         ZK_CUDA(cudaGetLastError());
-        launch_linear_base(sums.as<unsigned long long>(), src[2], src[3], w, base.as<uint32_t>(),
-                           status.as<uint32_t>(), s);
+        launch_linear_base(sums, src[2], src[3], w, base, status, s);
         ZK_CUDA(cudaGetLastError());
         ctx->launches += 2;
-        ZK_CUDA(cudaMemcpyAsync(st, status.ptr, 8, cudaMemcpyDeviceToHost, s));
+        ZK_CUDA(cudaMemcpyAsync(st, status, 8, cudaMemcpyDeviceToHost, s));
         ZK_CUDA(cudaStreamSynchronize(s));
         if (st[0] || st[1] <= w.planes) break;
     }
     *bad = st[0];
     w.tiles = tiles.as<uint8_t>();
-    w.base = base.as<uint32_t>();
+    w.base = base;
     return ZKML_OK;
 }
 
@@ -170,16 +172,15 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     zkml_linear* lin = new zkml_linear();
     struct Drop {
         zkml_linear*& l;
-        DevBuf stage[4], sums;
+        DevBuf stage[4];
         ~Drop() {  // cudaFree waits for the kernels that use these
             for (DevBuf& b : stage) b.release();
-            sums.release();
             if (l) {
                 l->release();
                 delete l;
             }
         }
-    } drop{lin, {}, {}};
+    } drop{lin, {}};
     lin->ctx = ctx;
     PackedWeights& w = lin->w;
     set_shape(w, k, n, parts == 2);
@@ -210,7 +211,7 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
         *to = drop.stage[g].as<uint32_t>();
     }
     uint32_t bad = 0;
-    if ((rc = lay_out(ctx, w, dev, rs, cs, lin->tiles, drop.sums, lin->base, lin->status, s, &bad))) return rc;
+    if ((rc = lay_out(ctx, w, dev, rs, cs, lin->tiles, lin->small, s, &bad))) return rc;
     if (bad) return set_error(ZKML_ERR_INVALID_ARG, "linear: weight or bias value >= 2^31 is not an M31 element");
     *out = lin;
     lin = nullptr;
@@ -219,17 +220,16 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
 
 }  // namespace
 
-// Words 4 and up of the scratch status collect what the calls meet; lay_out uses those before.
 int linear_once_begin(zkml_ctx* ctx) {
-    const int rc = ctx->lin.status.ensure(256);
+    const int rc = ctx->lin.met.ensure(4);
     if (rc) return rc;
-    ZK_CUDA(cudaMemsetAsync(ctx->lin.status.ptr, 0, 256, ctx->stream));
+    ZK_CUDA(cudaMemsetAsync(ctx->lin.met.ptr, 0, 4, ctx->stream));
     return ZKML_OK;
 }
 
 int linear_once_end(zkml_ctx* ctx) {
     uint32_t st = 0;
-    ZK_CUDA(cudaMemcpyAsync(&st, ctx->lin.status.as<uint32_t>() + 4, 4, cudaMemcpyDeviceToHost, ctx->stream));
+    ZK_CUDA(cudaMemcpyAsync(&st, ctx->lin.met.ptr, 4, cudaMemcpyDeviceToHost, ctx->stream));
     ZK_CUDA(cudaStreamSynchronize(ctx->stream));
     return status_error(st);
 }
@@ -247,7 +247,7 @@ int linear_once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint
     uint32_t bad = 0;
     int rc = device_view(ctx, w, k * n * 4, ctx->b_in, &dev);
     const uint32_t* src[4] = {static_cast<const uint32_t*>(dev), nullptr, nullptr, nullptr};
-    if (!rc) rc = lay_out(ctx, p, src, n, 1, b.tiles, b.sums, b.base, b.status, s, &bad);
+    if (!rc) rc = lay_out(ctx, p, src, n, 1, b.tiles, b.small, s, &bad);
     if (rc) return rc;
     if (bad) return set_error(ZKML_ERR_INVALID_ARG, "matmul_m31: input value >= 2^31 is not an M31 element");
     const Choice& c = choose(p, (uint32_t)m, 31, ctx->num_sms);
@@ -257,7 +257,7 @@ int linear_once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint
     io.residual = residual;
     io.out = out;
     io.pre = pre;
-    io.status = b.status.as<uint32_t>() + 4;
+    io.status = b.met.as<uint32_t>();
     io.ldx = k;
     io.ld_res = io.ld_out = io.ld_pre = n;
     io.m = (uint32_t)m;
@@ -353,7 +353,7 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     io.out = c->out;
     io.pre = c->pre;
     io.up = c->up;
-    io.status = lin->status.as<uint32_t>();
+    io.status = lin->small.as<uint32_t>();
     io.ldx = c->ldx;
     io.ld_res = c->ld_residual;
     io.ld_out = c->ld_out;
@@ -377,9 +377,9 @@ int zkml_linear_check(zkml_linear* lin, void* stream) {
     if (cap != cudaStreamCaptureStatusNone)
         return set_error(ZKML_ERR_INVALID_ARG, "the check waits for the stream, which is being captured");
     uint32_t st = 0;
-    ZK_CUDA(cudaMemcpyAsync(&st, lin->status.ptr, 4, cudaMemcpyDeviceToHost, s));
+    ZK_CUDA(cudaMemcpyAsync(&st, lin->small.ptr, 4, cudaMemcpyDeviceToHost, s));
     ZK_CUDA(cudaStreamSynchronize(s));
-    if (st) ZK_CUDA(cudaMemsetAsync(lin->status.ptr, 0, 4, s));
+    if (st) ZK_CUDA(cudaMemsetAsync(lin->small.ptr, 0, 4, s));
     return status_error(st);
 }
 

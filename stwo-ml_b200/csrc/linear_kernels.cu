@@ -41,48 +41,60 @@ __device__ __forceinline__ int planes_needed(int v) {
     return 4;
 }
 
-// One block per weight tile; a thread packs 16 consecutive K of one row per step (reads along the
-// rows of a row-major matrix are coalesced over the lanes, each store is one 16-byte chunk).
+// One block per weight tile.  A thread makes four 16-byte chunks of one row (16 consecutive K each;
+// reads along the rows of a row-major matrix are coalesced over the lanes), which pass through
+// shared memory so that a plane's tile is stored as one run of bytes: stored where they are made,
+// 16 bytes to each 128-byte row, 71 M weights took 159 us.
 __global__ void __launch_bounds__(256) linear_pack_kernel(const uint32_t* __restrict__ w, const uint32_t* __restrict__ w2,
                                                           size_t rs, size_t cs, PackedWeights p,
                                                           uint8_t* __restrict__ tiles,
                                                           unsigned long long* __restrict__ sums,
                                                           uint32_t* __restrict__ status) {
+    __shared__ __align__(16) uint4 stage[LIN_TILE_BYTES / 16];
     const uint32_t nt = blockIdx.x / p.k_tiles, kt = blockIdx.x % p.k_tiles;
+    const uint32_t r = threadIdx.x % LIN_ROWS, c0 = threadIdx.x / LIN_ROWS;  // chunks c0, c0 + 2, c0 + 4, c0 + 6
+    const uint32_t part = p.gated ? (r >> 4) & 1 : 0;
+    const uint32_t f = p.gated ? nt * 64 + (r >> 5) * 16 + (r & 15) : nt * LIN_ROWS + r;
+    const uint32_t* src = part ? w2 : w;
     uint32_t bad = 0;
     int need = 1;
-    for (uint32_t e = threadIdx.x; e < LIN_ROWS * 8; e += 256) {
-        const uint32_t r = e % LIN_ROWS, c = e / LIN_ROWS;
-        const uint32_t part = p.gated ? (r >> 4) & 1 : 0;
-        const uint32_t f = p.gated ? nt * 64 + (r >> 5) * 16 + (r & 15) : nt * LIN_ROWS + r;
-        const uint32_t* src = part ? w2 : w;
-        const uint32_t k0 = kt * LIN_KB + 16 * c;
-        uint32_t d[4][4] = {};
-        unsigned long long sum = 0;
-        if (f < p.n) {
+    unsigned long long sum = 0;
+    uint32_t d[4][4][4];  // [chunk][plane][word]
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                uint32_t q[4];
+    for (int h = 0; h < 4; h++) {
+        const uint32_t k0 = kt * LIN_KB + 16 * (c0 + 2 * h);
+        uint32_t v[16];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t at = k0 + 4 * i + j;
-                    const uint32_t v = at < p.k ? __ldg(src + (size_t)at * rs + (size_t)f * cs) : 0u;
-                    bad |= v >> 31;
-                    const int s = m31_signed(v);
-                    sum += (unsigned long long)(s < 0 ? s + (int)P : s);
-                    need = max(need, planes_needed(s));
-                    q[j] = balanced_digits(s);
-                }
-                byte_planes(make_uint4(q[0], q[1], q[2], q[3]), d[0][i], d[1][i], d[2][i], d[3][i]);
+        for (uint32_t j = 0; j < 16; j++)
+            v[j] = f < p.n && k0 + j < p.k ? __ldg(src + (size_t)(k0 + j) * rs + (size_t)f * cs) : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                bad |= v[4 * i + j] >> 31;
+                const int s = m31_signed(v[4 * i + j]);
+                sum += (unsigned long long)(s < 0 ? s + (int)P : s);
+                need = max(need, planes_needed(s));
+                q[j] = balanced_digits(s);
             }
+            byte_planes(make_uint4(q[0], q[1], q[2], q[3]), d[h][0][i], d[h][1][i], d[h][2][i], d[h][3][i]);
         }
-        const size_t plane = (size_t)p.n_tiles * p.k_tiles * LIN_TILE_BYTES;
-        uint8_t* dst = tiles + ((size_t)nt * p.k_tiles + kt) * LIN_TILE_BYTES + r * LIN_KB + ((c ^ (r & 7)) << 4);
-#pragma unroll
-        for (int b = 0; b < 4; b++)
-            if (b < (int)p.planes) *reinterpret_cast<uint4*>(dst + b * plane) = make_uint4(d[b][0], d[b][1], d[b][2], d[b][3]);
-        if (sum) atomicAdd(sums + (size_t)nt * LIN_ROWS + r, sum);
     }
+    const size_t plane = (size_t)p.n_tiles * p.k_tiles * LIN_TILE_BYTES;
+    uint4* dst = reinterpret_cast<uint4*>(tiles + ((size_t)nt * p.k_tiles + kt) * LIN_TILE_BYTES);
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        if (b >= (int)p.planes) break;
+        if (b) __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 4; h++)
+            stage[r * 8 + ((c0 + 2 * h) ^ (r & 7))] = make_uint4(d[h][b][0], d[h][b][1], d[h][b][2], d[h][b][3]);
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 4; h++) dst[b * (plane / 16) + threadIdx.x + 256 * h] = stage[threadIdx.x + 256 * h];
+    }
+    if (sum) atomicAdd(sums + (size_t)nt * LIN_ROWS + r, sum);
     if (bad) atomicOr(status, LIN_BAD_VALUE);
     if (need > 1) atomicMax(status + 1, (uint32_t)need);
 }
@@ -504,8 +516,8 @@ void launch_linear_base(const unsigned long long* sums, const uint32_t* bias, co
     linear_base_kernel<<<p.n_tiles, LIN_ROWS, 0, s>>>(sums, bias, bias2, p, base, status);
 }
 
-// Clocks of a split: a model with rates fitted to 389 measured splits of 22 calls (m 9 to 2048, K 500
-// to 13824; the split it picks is within 1 % of the fastest on average).  A block multiplies 128
+// Clocks of a split: a model with rates fitted to 562 measured splits of 22 calls (m 9 to 2048, K 500
+// to 13824; the split it picks is within 2 % of the fastest on average, 14 % at worst).  A block multiplies 128
 // rows x N columns x 128 K in 2 N clocks and takes in 48 bytes a clock, all blocks together 5300;
 // a token of a tile costs 50 clocks to finish, under the next tile's products except for the
 // last tile; cutting tiles costs a round through memory for the parts, 3500 clocks where every
@@ -544,21 +556,20 @@ LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_s
         const uint32_t waves = p.tiles / num_sms;
         // whole tiles only; the tiles beyond the last full wave but one cut over all blocks; with fewer
         // tiles than blocks, each cut into the same number of parts
-        for (int mode = 0; mode < 6; mode++) {
-            if (mode == 0) {
+        for (uint32_t parts = 0; parts <= 16; parts++) {  // 0: whole tiles, 1: straddling shares, else parts of a tile
+            if (parts == 0) {
                 p.ctas = std::min(p.tiles, (uint32_t)num_sms);
                 p.sk_tiles = 0;
-            } else if (mode == 1) {
+            } else if (parts == 1) {
                 p.ctas = (uint32_t)std::min<uint64_t>((uint64_t)num_sms, per_tile * p.tiles);
                 if (p.tiles % p.ctas == 0) continue;
                 p.sk_tiles = waves ? p.tiles - (waves - 1) * p.ctas : p.tiles;
             } else {
-                const uint32_t parts = 1u << (mode - 1);
                 if (parts > per_tile || (uint64_t)p.tiles * parts > (uint64_t)num_sms) break;
                 p.ctas = p.tiles * parts;
                 p.sk_tiles = p.tiles;
             }
-            const double c = plan_clocks(p, per_tile, m, mode == 1);
+            const double c = plan_clocks(p, per_tile, m, parts == 1);
             if (!best.tiles || c < best_clocks) best = p, best_clocks = c;
         }
     }

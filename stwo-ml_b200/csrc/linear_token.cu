@@ -22,12 +22,16 @@ constexpr uint32_t MAKERS = 8;  // warps that make digit tiles; four of them fin
 constexpr uint32_t TOKEN_THREADS = 64 + 32 * MAKERS;
 constexpr uint32_t TOKEN_SMEM = 110 * 1024;  // two blocks an SM
 constexpr uint32_t MAX_STAGES = 6;
+constexpr uint32_t MAX_TOKENS = 8;
+constexpr uint32_t MAX_COLS = 32;                // digit columns
+constexpr uint32_t GROUPS = MAX_COLS / 16;       // token groups a thread finishes, at most
 
 struct TokenArgs {
     PackedWeights w;
     LinearIO io;
     const uint32_t* base;
     uint32_t tokens, parts, stages;
+    uint32_t slices;  // warps that share a unit's tokens: 1, 2 or 4
 };
 
 template <int D, bool GATED>
@@ -53,7 +57,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
     if (threadIdx.x == 0) {
         quit_s = 0;
         for (uint32_t i = 0; i < a.stages; i++) {
-            mbar_init(full + 8 * i, 2);  // the copy's issuer and the digit maker
+            mbar_init(full + 8 * i, 1 + a.slices);  // the copy's issuer and the digit makers
             mbar_init(empty + 8 * i, 1);
         }
         mbar_init(acc_full, 1);
@@ -75,8 +79,8 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         plane = u / k_len;
         kt = k_begin + u - plane * k_len;
     };
-    // accumulators of this thread's row, joined over digits and planes, for up to 2 groups of tokens
-    uint32_t z[2][G];
+    // accumulators of this thread's row, joined over digits and planes, group by group
+    uint32_t z[GROUPS][G];
     const uint32_t quad = warp & 3, row = quad * 32 + lane;
     bool ok = true;
 
@@ -129,66 +133,65 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             }
         }
     } else {
-        // ---- digit tiles: each warp makes those of every makers-th unit; a lane takes 4 K of every token
+        // ---- digit tiles: a lane takes 4 K of a token
         grid_dependency_wait();
-        // no more makers than stages: a maker is then never two uses of a stage ahead of its barrier
-        const uint32_t maker = warp - 2, makers = min(MAKERS, a.stages);
+        // A unit's tokens are dealt to `slices` warps, at most two to each, and the units to the
+        // 8 / slices groups of warps; no more groups than stages, so that a group is never two uses of a
+        // stage ahead of its barrier.
+        const uint32_t maker = warp - 2, slice = maker % a.slices, groups = min(MAKERS / a.slices, a.stages);
         const bool vec = (a.io.ldx % 4 == 0) && ((reinterpret_cast<uintptr_t>(a.io.x) & 15) == 0);
         uint32_t bad = 0;
-        // 4 tokens at a time; the next ones' words are on their way while these become digits
-        const auto load = [&](uint4(&v)[4], uint32_t u, uint32_t t0) {
+        const auto load = [&](uint4(&v)[2], uint32_t u) {
             uint32_t plane, kt;
             tile_of(u, plane, kt);
             const uint32_t k0 = kt * LIN_KB + 4 * lane;
 #pragma unroll
-            for (uint32_t t = 0; t < 4; t++) {
-                v[t] = make_uint4(0, 0, 0, 0);
-                if (t0 + t >= a.io.m) continue;
-                const uint32_t* src = a.io.x + (size_t)(t0 + t) * a.io.ldx + k0;
+            for (uint32_t i = 0; i < 2; i++) {
+                const uint32_t t = slice + i * a.slices;
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (t >= a.io.m) continue;
+                const uint32_t* src = a.io.x + (size_t)t * a.io.ldx + k0;
                 if (vec && k0 + 4 <= a.w.k) {
-                    v[t] = __ldg(reinterpret_cast<const uint4*>(src));
+                    v[i] = __ldg(reinterpret_cast<const uint4*>(src));
                 } else {
-                    if (k0 < a.w.k) v[t].x = __ldg(src);
-                    if (k0 + 1 < a.w.k) v[t].y = __ldg(src + 1);
-                    if (k0 + 2 < a.w.k) v[t].z = __ldg(src + 2);
-                    if (k0 + 3 < a.w.k) v[t].w = __ldg(src + 3);
+                    if (k0 < a.w.k) v[i].x = __ldg(src);
+                    if (k0 + 1 < a.w.k) v[i].y = __ldg(src + 1);
+                    if (k0 + 2 < a.w.k) v[i].z = __ldg(src + 2);
+                    if (k0 + 3 < a.w.k) v[i].w = __ldg(src + 3);
                 }
             }
         };
-        uint32_t u = maker < makers ? maker : units, t0 = 0;
-        uint4 v[4], ahead[4];
-        if (u < units) load(v, u, 0);
+        uint32_t u = maker / a.slices < groups ? maker / a.slices : units;
+        uint4 v[2], ahead[2];
+        if (u < units) load(v, u);
         while (u < units) {
-            const uint32_t t_next = t0 + 4 < a.io.m ? t0 + 4 : 0, u_next = t_next ? u : u + makers;
-            if (u_next < units) load(ahead, u_next, t_next);
+            const uint32_t u_next = u + groups;
+            if (u_next < units) load(ahead, u_next);  // on its way while this one becomes digits
             const uint32_t st = u % a.stages, tile = smem0 + st * stage_bytes + LIN_TILE_BYTES;
-            if (t0 == 0) {  // the stage's last product is done
-                ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ((u / a.stages) & 1) ^ 1, &quit_s));
-                if (!ok) break;
-            }
+            // the stage's last product is done
+            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ((u / a.stages) & 1) ^ 1, &quit_s));
+            if (!ok) break;
 #pragma unroll
-            for (uint32_t t = 0; t < 4; t++) {
-                if (t0 + t >= a.io.m) continue;
+            for (uint32_t i = 0; i < 2; i++) {
+                const uint32_t t = slice + i * a.slices;
+                if (t >= a.io.m) continue;
                 uint32_t d[D];
-                activation_digits<D>(v[t], d, bad);
+                activation_digits<D>(v[i], d, bad);
 #pragma unroll
                 for (int b = 0; b < D; b++) {
-                    const uint32_t r = b * a.tokens + t0 + t;
+                    const uint32_t r = b * a.tokens + t;
                     asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile + r * LIN_KB + (((lane >> 2) ^ (r & 7)) << 4) +
                                                                 4 * (lane & 3)),
                                  "r"(d[b])
                                  : "memory");
                 }
             }
-            if (t_next == 0) {
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full + 8 * st);
-            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full + 8 * st);
             u = u_next;
-            t0 = t_next;
 #pragma unroll
-            for (int t = 0; t < 4; t++) v[t] = ahead[t];
+            for (int i = 0; i < 2; i++) v[i] = ahead[i];
         }
         if (bad) atomicOr(a.io.status, bad);
         // ---- this warp's quarter of the rows (warps 2 to 5): TMEM lanes 32 (warp % 4) and up
@@ -197,7 +200,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             tc_fence_after();
             if (ok) {
 #pragma unroll
-                for (uint32_t h = 0; h < 2; h++) {
+                for (uint32_t h = 0; h < GROUPS; h++) {
                     if (h * G >= a.tokens) break;
                     for (uint32_t plane = 0; plane < a.w.planes; plane++) {
                         const uint32_t acc = tmem + plane * n_cols + h * G + ((quad * 32) << 16);
@@ -229,7 +232,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         if (finisher && ok) {
             const uint32_t at = part_base + ((rank * held + quad / holders) * a.tokens * 32 + lane) * 4;
 #pragma unroll
-            for (uint32_t h = 0; h < 2; h++)
+            for (uint32_t h = 0; h < GROUPS; h++)
 #pragma unroll
                 for (uint32_t t = 0; t < G; t++)
                     if (h * G + t < a.io.m) cluster_store(at + (h * G + t) * 128, quad % holders, z[h][t]);
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         cluster_wait();
         if (finisher && ok && quad % holders == rank) {
 #pragma unroll
-            for (uint32_t h = 0; h < 2; h++) {
+            for (uint32_t h = 0; h < GROUPS; h++) {
                 if (h * G >= a.io.m) break;
                 uint64_t sum[G];
 #pragma unroll
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         }
     } else if (finisher && ok) {
 #pragma unroll
-        for (uint32_t h = 0; h < 2; h++) {
+        for (uint32_t h = 0; h < GROUPS; h++) {
             if (h * G >= a.io.m) break;
             finish_tokens<D, GATED>(a.io, a.w.n, nt, row, h * G, base, z[h]);
         }
@@ -298,14 +301,14 @@ cudaError_t linear_token_configure() {
     return cudaSuccess;
 }
 
-// Taken for up to 16 tokens and 32 digit columns (8 tokens of 31 bits): beyond, making the digits
-// once for all weight tiles is cheaper than in every block (32 int8 tokens x 5120 x 5120: 28.6
-// against 20.5 us; 16: 16.2 against 18.8).
+// Taken for up to 8 tokens: beyond, making the digits once for all weight tiles is cheaper than in
+// every block (31-bit tokens x 5120 x 13824: 8 tokens 17.8 us here, 17.9 us with a digit kernel; 12
+// tokens 23.5 against 17.8 us; x 5120 x 5120: 10.6 against 13.4, 13.8 against 13.6 us).
 bool linear_token_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms, TokenPlan* out) {
     TokenPlan p{};
     p.digits = x_bits == 8 ? 1 : x_bits == 16 ? 2 : 4;
     const uint32_t n_cols = m * p.digits <= 16 ? 16 : 32;
-    if (m > 16 || m * p.digits > n_cols) return false;
+    if (m > MAX_TOKENS) return false;
     p.tokens = n_cols / p.digits;
     // As many blocks to a cluster as stay resident at once, two an SM less a tenth that clusters cannot
     // fill, up to 6 (one token, 5120 x 5120: 15.8 us with 1, 11.1 with 2, 8.3 with 4, 8.1 with 5, 8.2 with 6;
@@ -332,6 +335,7 @@ cudaError_t launch_linear_token(const PackedWeights& w, const TokenPlan& p, cons
     a.tokens = p.tokens;
     a.parts = p.parts;
     a.stages = p.stages;
+    a.slices = io.m <= 2 ? 1 : io.m <= 4 ? 2 : 4;
     return p.digits == 1   ? launch<1>(a, p, s, overlap)
            : p.digits == 2 ? launch<2>(a, p, s, overlap)
                            : launch<4>(a, p, s, overlap);
