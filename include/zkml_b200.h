@@ -414,7 +414,8 @@ int zkml_linear_create(zkml_ctx *ctx, const uint32_t *w, size_t k, size_t n, siz
 int zkml_linear_create_gated(zkml_ctx *ctx, const uint32_t *w_gate, const uint32_t *w_up, size_t k, size_t n,
                              size_t row_stride, size_t col_stride, const uint32_t *bias_gate,
                              const uint32_t *bias_up, void *stream, zkml_linear **out);
-/* Waits for the work that uses the weights.  NULL is fine. */
+/* Waits for the work that uses the weights.  CUDA graphs that captured calls must not be replayed
+ * afterwards.  NULL is fine. */
 int zkml_linear_destroy(zkml_linear *lin);
 
 /* One call.  All pointers are memory of the context's GPU, strides are in words.  A row of x or

@@ -8,6 +8,7 @@
 
 struct zkml_linear {
     zkml_ctx* ctx = nullptr;
+    int device = 0;
     zk::PackedWeights w;
     zk::DevBuf tiles;
     zk::DevBuf small;  // status words, column sums, per-row constants
@@ -182,6 +183,7 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
         }
     } drop{lin, {}};
     lin->ctx = ctx;
+    lin->device = ctx->device;
     PackedWeights& w = lin->w;
     set_shape(w, k, n, parts == 2);
     const uint32_t* dev[4] = {};  // weights, then biases
@@ -288,8 +290,12 @@ int zkml_linear_create_gated(zkml_ctx* ctx, const uint32_t* w_gate, const uint32
 
 int zkml_linear_destroy(zkml_linear* lin) {
     if (!lin) return ZKML_OK;
-    DeviceGuard guard(lin->ctx->device);
+    DeviceGuard guard(lin->device);
+    // a destructor may run while some stream of the program is captured: freeing is no part of that capture
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     lin->release();  // cudaFree waits for the work that reads the weights
+    cudaThreadExchangeStreamCaptureMode(&mode);
     delete lin;
     return ZKML_OK;
 }

@@ -354,6 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
             Schedule sch;
             sch.init(a);
             Segment s{};
+            grid_dependency_wait();  // so that the waits' limit counts this grid's own time alone
             const uint32_t idesc = tc_idesc_s8(n_cols);
             uint32_t st = 0, phase = 0, seg = 0;
             bool ok = true;

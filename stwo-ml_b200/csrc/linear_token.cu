@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         if (lane == 0) {
             uint32_t st = 0, phase = 1, issued = 0;
             for (uint32_t u = 0; u < units; u++) {
+                if (u == a.stages) grid_dependency_wait();  // so that the waits' limit counts this grid's own time alone
                 if (!(ok = mbar_wait(empty + 8 * st, phase, &quit_s))) break;
                 uint32_t plane, kt;
                 tile_of(u, plane, kt);
@@ -109,6 +110,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         }
     } else if (warp == 1) {
         if (lane == 0) {
+            grid_dependency_wait();
             const uint32_t idesc = tc_idesc_s8(n_cols);
             uint32_t st = 0, phase = 0, kt_done = 0, plane = 0;
             for (uint32_t u = 0; u < units; u++) {

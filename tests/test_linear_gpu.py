@@ -421,3 +421,63 @@ def test_equal_results_on_every_run():
     first = lin(x)
     for _ in range(20):
         assert torch.equal(lin(x), first)
+
+
+def test_handles_closed_while_work_is_queued_and_while_capturing():
+    """Closing waits for the calls that read the weights, and is no part of another handle's capture."""
+    x, w = ints((300, 2000), 31, 1), ints((2000, 500), 8, 2)
+    tx, tw, want = dev(x), dev(w), L.product(x, w)
+    outs = []
+    for _ in range(5):
+        lin = Z.LinearM31(tw)
+        outs += [lin(tx, check=False) for _ in range(3)]
+        lin.close()
+    torch.cuda.synchronize()
+    for o in outs:
+        L.same(host(o), want)
+    lin, other = Z.LinearM31(tw), Z.LinearM31(tw)
+    lin(tx)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = lin(tx, check=False)
+        other.close()
+    g.replay()
+    torch.cuda.synchronize()
+    L.same(host(y), want)
+    lin.check()
+
+
+def test_a_call_behind_long_and_mixed_work():
+    """Calls of every size in one stream, each reading the one before: nothing is read too early."""
+    d = 640
+    ws = [ints((d, d), 8, i) for i in range(3)]
+    ops = [Z.LinearM31(dev(w)) for w in ws]
+    x = ints((200, d), 31, 9)
+    tx, y = dev(x), x
+    torch.cuda._sleep(20_000_000)
+    cur = tx
+    for i, m in enumerate((200, 200, 40, 40, 8, 8, 1, 1)):
+        cur = ops[i % 3](cur[:m], residual=cur[:m], check=False)
+        y = L.linear(y[:m], ws[i % 3], None, 0, y[:m])[0]
+    torch.cuda.synchronize()
+    L.same(host(cur), y)
+
+
+def test_two_threads_share_a_handle():
+    import threading
+    x, w = ints((50, 700), 31, 1), ints((700, 300), 8, 2)
+    lin, want, tx = Z.LinearM31(dev(w)), L.product(x, w), dev(x)
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = [lin(tx[:1 + 7 * i], check=False) for _ in range(30)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for i, outs in got.items():
+        for o in outs:
+            L.same(host(o), want[:1 + 7 * i])
