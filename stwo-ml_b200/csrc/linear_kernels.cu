@@ -517,24 +517,24 @@ void launch_linear_base(const unsigned long long* sums, const uint32_t* bias, co
     linear_base_kernel<<<p.n_tiles, LIN_ROWS, 0, s>>>(sums, bias, bias2, p, base, status);
 }
 
-// Clocks of a split: a model with rates fitted to 562 measured splits of 22 calls (m 9 to 2048, K 500
-// to 13824; the split it picks is within 2 % of the fastest on average, 14 % at worst).  A block multiplies 128
-// rows x N columns x 128 K in 2 N clocks and takes in 48 bytes a clock, all blocks together 5300;
-// a token of a tile costs 50 clocks to finish, under the next tile's products except for the
-// last tile; cutting tiles costs a round through memory for the parts, 3500 clocks where every
-// tile has the same number of parts and 10000 where shares straddle tiles.
+// Clocks of a split: a model with rates fitted to 916 measured splits of 33 calls (m 9 to 2048, K 300
+// to 13824; the split it picks takes 2 % longer than the fastest on average, 13 % at worst).  A block
+// multiplies 128 rows x N columns x 128 K in 2 N clocks and takes in 46 bytes a clock, all blocks
+// together 5500; a token of a tile costs 30 clocks to finish, under the next tile's products
+// except for the last tile; cutting tiles costs a round through memory for the parts, 5200 clocks
+// where every tile has the same number of parts and 9300 where shares straddle tiles.
 static double plan_clocks(const LinearPlan& p, uint64_t per_tile, uint32_t m, bool straddles) {
     const double n_cols = (double)p.digits * p.tokens, live = std::min(m, p.tokens);
-    const double bytes = LIN_TILE_BYTES + n_cols * LIN_KB, unit = std::max(2.0 * n_cols, bytes / 48.0);
-    const double finish = 900 + 50.0 * live, tile = unit * per_tile;
+    const double bytes = LIN_TILE_BYTES + n_cols * LIN_KB, unit = std::max(2.0 * n_cols, bytes / 46.0);
+    const double finish = 1800 + 30.0 * live, tile = unit * per_tile;
     const uint32_t whole = (p.tiles - p.sk_tiles + p.ctas - 1) / p.ctas;
     double t = whole ? whole * std::max(tile, finish) + finish : 0;
     if (p.sk_tiles) {
         const double tiles = (double)p.sk_tiles / p.ctas, share = tiles * per_tile;
         const double parts = per_tile / share + (straddles ? 1 : 0), pieces = straddles ? tiles + 1 : 1;
-        t += share * unit + (straddles ? 10000 : 3500) + pieces * live * 57 + std::max(1.0, tiles) * live * (50 + 22 * parts);
+        t += share * unit + (straddles ? 9300 : 5200) + pieces * live * 76 + std::max(1.0, tiles) * live * (30 + 19 * parts);
     }
-    return std::max(t, (double)p.tiles * per_tile * bytes / 5300 + finish);
+    return std::max(t, (double)p.tiles * per_tile * bytes / 5500 + finish);
 }
 
 LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_sms) {
