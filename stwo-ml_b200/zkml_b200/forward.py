@@ -47,15 +47,18 @@ def _is_tensor(x) -> bool:
     return hasattr(x, "data_ptr") and hasattr(x, "is_cuda")
 
 
+_torch_module = None
+
+
 def _torch():
-    import torch
+    global _torch_module
+    if _torch_module is None:
+        import torch
 
-    if _i32[0] is None:
-        _i32[0] = torch.int32
-    return torch
+        _torch_module = torch
+    return _torch_module
 
 
-_i32 = [None]  # torch.int32, once torch is there
 _forward_fn = []
 
 
@@ -143,7 +146,7 @@ class _Weights:
 
     def _rows(self, x, width, name, m=None):
         """(pointer, rows, row stride) of a matrix of words on this device; one row may be 1-D."""
-        if x.dtype is _i32[0] and x.is_cuda and x.device.index == self.device and x.dim() == 2:
+        if x.is_cuda and x.dtype is _torch().int32 and x.get_device() == self.device and x.dim() == 2:
             rows, cols = x.shape
             ld, one = x.stride()
             if cols == width and (one == 1 or width == 1) and rows and (m is None or rows == m):
@@ -183,7 +186,7 @@ class _Weights:
         if out is None or (keep and (pre is None or (up is None and self._gated))):
             shape = (*x.shape[:-1], n)
         if out is None:
-            out = torch.empty(shape, dtype=torch.int32, device=x.device)
+            out = x.new_empty(shape, dtype=torch.int32)
             op, ldo = out.data_ptr(), n
         else:
             op, _, ldo = self._rows(out, n, "out", m)
@@ -191,14 +194,14 @@ class _Weights:
         if pre is not None:
             pp, _, ldp = self._rows(pre, n, "pre", m)
         elif keep:
-            pre = torch.empty(shape, dtype=torch.int32, device=x.device)
+            pre = x.new_empty(shape, dtype=torch.int32)
             pp, ldp = pre.data_ptr(), n
         if pre is not None:
             results.append(pre)
         if up is not None:
             pu, _, ldu = self._rows(up, n, "up", m)
         elif keep and self._gated:
-            up = torch.empty(shape, dtype=torch.int32, device=x.device)
+            up = x.new_empty(shape, dtype=torch.int32)
             pu, ldu = up.data_ptr(), n
         if up is not None:
             results.append(up)
@@ -210,12 +213,14 @@ class _Weights:
                 self._need.clear()
             need = self._need[(m, x_bits)] = size.value
         if need:
-            keep_ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-            ws = keep_ws.data_ptr()
+            workspace = x.new_empty(need, dtype=torch.uint8)
+            ws = workspace.data_ptr()
         stream = torch._C._cuda_getCurrentRawStream(self.device) or _STREAM_LEGACY
         call = _CALL.pack(xp, m, ldx, int(x_bits), _tag(activation), rp, ldr, op, ldo, pp, ldp, pu, ldu, ws, need, stream,
                           1)
-        _check(_forward()(self._handle.value, call))
+        rc = _forward()(self._handle.value, call)
+        if rc:
+            _check(rc)
         if check:
             self.check()
         return results
@@ -226,7 +231,7 @@ class _Weights:
         _check(lib().zkml_linear_check(self._handle, self._stream()))
 
     def _run(self, x, activation, residual, out, pre, up, keep, x_bits, check):
-        if _is_tensor(x):
+        if x.__class__ is _torch().Tensor or _is_tensor(x):
             r = self._call(x, activation, residual, out, pre, up, keep, x_bits, check)
             return r[0] if len(r) == 1 else tuple(r)
         if out is not None or pre is not None or up is not None:
