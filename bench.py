@@ -936,6 +936,17 @@ def run_case(name):
         g = (np.arange(cols, dtype=np.uint32) % 1000) + 1
         for _ in range(2):
             Z.reduce_rmsnorm_layer(Z.GKRClaim(pt, val), Z.M31Matrix.from_numpy(x), cols, Z.PoseidonChannel(), gamma=g)
+    elif name.startswith(("linear_", "gated_")):  # forward operator m x k x n (e.g. linear_64x5120x13824), three times
+        m_, k_, n_ = (int(v) for v in name.split("_")[1].split("x"))
+        gated = name.startswith("gated_")
+        ws = []
+        for _ in range(2 if gated else 1):
+            w_ = torch.randint(-127, 128, (k_, n_), dtype=torch.int32, device="cuda")
+            ws.append(torch.where(w_ < 0, w_ + (2**31 - 1), w_))
+        x = torch.randint(0, 2**31 - 1, (m_, k_), dtype=torch.int32, device="cuda")
+        op = (Z.GatedLinearM31 if gated else Z.LinearM31)(*ws)
+        for _ in range(3):
+            op(x, activation="silu")
     elif name.startswith("gemm_"):  # forward M31 GEMM M x K x N (e.g. gemm_64x5120x13824), three times
         m_, k_, n_ = (int(v) for v in name.split("_")[1].split("x"))
         a = torch.randint(-127, 128, (m_, k_), dtype=torch.int32, device="cuda")
