@@ -1,5 +1,7 @@
 // C-ABI: forward operators with weights laid out once (zkml_linear_*).
 #include <algorithm>
+#include <atomic>
+#include <new>
 #include <string>
 
 #include "context.hpp"
@@ -120,8 +122,12 @@ int lay_out(zkml_ctx* ctx, PackedWeights& w, const uint32_t* const src[4], size_
             DevBuf& small, cudaStream_t s, uint32_t* bad) {
     const size_t slots = (size_t)w.n_tiles * LIN_ROWS, plane = (size_t)w.n_tiles * w.k_tiles * LIN_TILE_BYTES;
     int rc;
-    ZK_CUDA(linear_configure());
-    ZK_CUDA(linear_token_configure());
+    static std::atomic<bool> configured[64];
+    if (ctx->device >= 64 || !configured[ctx->device].load(std::memory_order_relaxed)) {
+        ZK_CUDA(linear_configure());
+        ZK_CUDA(linear_token_configure());
+        if (ctx->device < 64) configured[ctx->device].store(true, std::memory_order_relaxed);
+    }
     if ((rc = small.ensure(STATUS_BYTES + slots * 16))) return rc;
     uint32_t* const status = small.as<uint32_t>();
     unsigned long long* const sums = reinterpret_cast<unsigned long long*>(small.as<uint8_t>() + STATUS_BYTES);
@@ -170,7 +176,8 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     ZK_CUDA(cudaStreamIsCapturing(s, &cap));
     if (cap != cudaStreamCaptureStatusNone)
         return set_error(ZKML_ERR_INVALID_ARG, "weights cannot be laid out while the stream is captured");
-    zkml_linear* lin = new zkml_linear();
+    zkml_linear* lin = new (std::nothrow) zkml_linear();
+    if (!lin) return set_error(ZKML_ERR_OOM, "no host memory for the handle");
     struct Drop {
         zkml_linear*& l;
         DevBuf stage[4];
@@ -238,9 +245,9 @@ int linear_once_end(zkml_ctx* ctx) {
 
 int linear_once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint32_t* w, size_t n, int activation,
                 const uint32_t* residual, uint32_t* pre, uint32_t* out) {
-    if (m > (1u << 30) || k > (1u << 30) || n > (1u << 30) || m * k > ((size_t)1 << 34) || k * n > ((size_t)1 << 34) ||
-        m * n > ((size_t)1 << 34))
+    if (m > (1u << 30) || k > (1u << 30) || n > (1u << 30) || m * k > ((size_t)1 << 34) || k * n > ((size_t)1 << 34))
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
+    if (m * n > ((size_t)1 << 34)) return set_error(ZKML_ERR_OOM, "output too large to be tiled");
     LinearScratch& b = ctx->lin;
     cudaStream_t s = ctx->stream;
     const void* dev = nullptr;

@@ -141,7 +141,8 @@ __device__ __forceinline__ void finish_tokens(const LinearIO& io, uint32_t n, ui
         if (f >= n) return;
         uint32_t res[G], bad = 0;
 #pragma unroll
-        for (int t = 0; t < G; t++) res[t] = io.residual && tok0 + t < io.m ? io.residual[(size_t)(tok0 + t) * io.ld_res + f] : 0u;
+        for (int t = 0; t < G; t++)
+            res[t] = io.residual && tok0 + t < io.m ? __ldcg(io.residual + (size_t)(tok0 + t) * io.ld_res + f) : 0u;
 #pragma unroll
         for (int t = 0; t < G; t++) {
             if (tok0 + t >= io.m) continue;

@@ -136,13 +136,13 @@ __global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* __re
     const uint32_t t = blockIdx.y * 32 + threadIdx.x / 8, c = threadIdx.x % 8;
     if (t < tokens) {
         const uint32_t row = mt * tokens + t, k0 = kt * LIN_KB + 16 * c;
-        uint4 v[4];
+        uint4 v[4];  // from L2: earlier work may have written x since this grid's blocks started
         const uint32_t* src = x + (size_t)row * ldx + k0;
         if (row < m && vec && k0 + 16 <= k) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+            for (int i = 0; i < 4; i++) v[i] = __ldcg(reinterpret_cast<const uint4*>(src) + i);
         } else {
-            const auto at = [&](uint32_t i) { return row < m && k0 + i < k ? __ldg(src + i) : 0u; };
+            const auto at = [&](uint32_t i) { return row < m && k0 + i < k ? __ldcg(src + i) : 0u; };
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) v[i] = make_uint4(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));
         }

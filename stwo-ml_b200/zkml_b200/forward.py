@@ -87,14 +87,12 @@ class _Weights:
             if tuple(w.shape) != tuple(first.shape):
                 raise InvalidArgument(1, "the weights of a gated block have the same shape")
         if any(_strides(w) != _strides(first) for w in weights):
-            weights = [w.contiguous() if _is_tensor(w) else w for w in weights]
+            weights = [w.contiguous() if _is_tensor(w) else np.ascontiguousarray(w) for w in weights]
         for w in weights:
             w = self._words(w, "weight")
             keep.append(w)
             ptrs.append(_pointer(w))
             strides.append(_strides(w))
-        if strides[0] != strides[-1]:
-            raise InvalidArgument(1, "the weights of a gated block are both tensors or both arrays")
         self.k, self.n = int(first.shape[0]), int(first.shape[1])
         for b in biases:
             if b is None:

@@ -227,7 +227,8 @@ def test_transposed_host_and_strided_weights():
         L.same(host(Z.LinearM31(weight)(dev(x))), want)
     h, _, _, unsure = L.gated(x, w, w[:, ::-1])
     up = np.ascontiguousarray(w[:, ::-1])
-    L.same(host(Z.GatedLinearM31(dev(w), dev(up.T).t())(dev(x))), h, unsure)
+    for gate_up in ((dev(w), dev(up.T).t()), (w, np.asfortranarray(up)), (w, np.flip(np.ascontiguousarray(np.flip(up)))), (dev(w), up), (w, dev(up))):
+        L.same(host(Z.GatedLinearM31(*gate_up)(dev(x))), h, unsure)
 
 
 def test_shapes_of_more_dimensions_and_arrays():
