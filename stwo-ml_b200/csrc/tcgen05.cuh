@@ -58,11 +58,6 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 
 // Thread-block clusters: a barrier of all threads of all blocks in two halves, and a store to the
 // same shared-memory address of another block.
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_store(uint32_t addr, uint32_t rank, uint32_t v) {

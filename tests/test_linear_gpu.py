@@ -243,6 +243,9 @@ def test_shapes_of_more_dimensions_and_arrays():
     out = torch.zeros(30, dtype=torch.int32, device="cuda")
     lin(dev(x)[3], out=out)
     L.same(host(out), want[3])
+    got = lin(dev(x).view(torch.uint32))
+    assert got.dtype == torch.int32
+    L.same(host(got), want)
 
 
 def test_bad_words_are_reported_once():
@@ -482,3 +485,35 @@ def test_two_threads_share_a_handle():
     for i, outs in got.items():
         for o in outs:
             L.same(host(o), want[:1 + 7 * i])
+
+
+@pytest.mark.parametrize("m,k,n", [(270001, 20, 8001), (600001, 4099, 3)])
+def test_offsets_past_32_bits(m, k, n):
+    """More than 2^31 words of output, of input and of digits: the first and last rows are right."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randint(0, P, (m, k), generator=g, device="cuda", dtype=torch.int32)
+    w = ints((k, n), 8, 2)
+    y = Z.LinearM31(dev(w))(x)
+    for rows in (slice(0, 70), slice(m // 2, m // 2 + 70), slice(m - 70, m)):
+        L.same(host(y[rows].contiguous()), L.product(host(x[rows].contiguous()), w))
+
+
+def test_many_drawn_calls():
+    """Sizes, widths, epilogues and strides drawn at random."""
+    rng = np.random.default_rng(11)
+    for i in range(60):
+        m, k, n = (int(round(2 ** rng.uniform(0, top))) for top in (8, 10, 9))
+        xb, wb = int(rng.choice([8, 16, 31])), int(rng.choice([8, 8, 16, 24, 31]))
+        act = str(rng.choice(list(TAGS)))
+        x, w, w2 = ints((m, k), xb, i), ints((k, n), wb, i + 1), ints((k, n), wb, i + 2)
+        b, r = ints((n,), 31, i + 3), ints((m, n), 31, i + 4)
+        px = torch.zeros(m, k + int(rng.integers(0, 5)), dtype=torch.int32, device="cuda")[:, :k]
+        px.copy_(dev(x))
+        y, z, unsure = L.linear(x, w, b, TAGS[act], r)
+        got = Z.LinearM31(dev(w), bias=dev(b))(px, activation=act, residual=dev(r), keep=True, x_bits=xb)
+        L.same(host(got[0]), y, unsure)
+        L.same(host(got[1]), z)
+        h, g, u, unsure = L.gated(x, w, w2, b, None, TAGS[act])
+        got = Z.GatedLinearM31(dev(w), dev(w2), bias_gate=dev(b))(px, activation=act, keep=True, x_bits=xb)
+        for a, want in zip(got, (h, g, u)):
+            L.same(host(a), want, unsure if want is h else None)
