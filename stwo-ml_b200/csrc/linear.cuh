@@ -39,6 +39,21 @@ void launch_linear_pack(const uint32_t* w, const uint32_t* w2, size_t rs, size_t
 void launch_linear_base(const unsigned long long* sums, const uint32_t* bias, const uint32_t* bias2,
                         const PackedWeights& p, uint32_t* base, uint32_t* status, cudaStream_t s);
 
+#ifdef __CUDACC__
+#define LIN_HD __host__ __device__
+#else
+#define LIN_HD
+#endif
+// Segment tables of SiLU and GELU (linear_act.cpp): by how much f falls short of max(x, 0) for the words
+// below act_limit (real x = 16 and 5), in segments of 2^act_segment_bits words, a record of 16 bytes
+// {c0, c1, c2, c3} each.
+LIN_HD constexpr uint32_t act_limit(int tag) { return tag == 2 ? 5u << 16 : 16u << 16; }
+LIN_HD constexpr uint32_t act_segment_bits(int tag) { return tag == 2 ? 10 : 11; }
+LIN_HD constexpr uint32_t act_table_bytes(int tag) { return 16 * (act_limit(tag) >> act_segment_bits(tag)); }
+constexpr uint32_t ACT_TABLE_MAX = 8192;
+static_assert(act_table_bytes(2) <= ACT_TABLE_MAX && act_table_bytes(5) <= ACT_TABLE_MAX, "reserved in the kernels");
+const uint8_t* act_segment_table(int tag);  // host; tag 2 or 5
+
 // One call.  Strides are in words.
 struct LinearIO {
     const uint32_t* x;
@@ -48,6 +63,7 @@ struct LinearIO {
     size_t ldx, ld_res, ld_out, ld_pre, ld_up;
     uint32_t m;
     int activation;
+    const uint8_t* act_table = nullptr;  // SiLU, GELU: the segment table in device memory
     bool as_reference = false;  // an activation that rounds a negative value to zero gives the word P, not 0
 };
 
@@ -76,6 +92,8 @@ cudaError_t launch_linear_token(const PackedWeights& w, const TokenPlan& p, cons
                                 bool overlap);
 cudaError_t linear_token_configure();
 cudaError_t linear_configure();  // per device, before the first launch
+// The current device's copy of the segment table, NULL for other activations.
+cudaError_t linear_act_table(int tag, const uint8_t** out);
 // overlap: the weights were in place before the work now queued on s, so they may be read while
 // that work still runs.
 cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const LinearIO& io, void* workspace,

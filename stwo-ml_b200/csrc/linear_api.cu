@@ -12,6 +12,7 @@ struct zkml_linear {
     zkml_ctx* ctx = nullptr;
     int device = 0;
     zk::PackedWeights w;
+    const uint8_t* act_table[2] = {nullptr, nullptr};  // GELU, SiLU: on the device
     zk::DevBuf tiles;
     zk::DevBuf small;  // status words, column sums, per-row constants
     void release() {
@@ -222,6 +223,8 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     uint32_t bad = 0;
     if ((rc = lay_out(ctx, w, dev, rs, cs, lin->tiles, lin->small, s, &bad))) return rc;
     if (bad) return set_error(ZKML_ERR_INVALID_ARG, "linear: weight or bias value >= 2^31 is not an M31 element");
+    ZK_CUDA(linear_act_table(2, &lin->act_table[0]));
+    ZK_CUDA(linear_act_table(5, &lin->act_table[1]));
     *out = lin;
     lin = nullptr;
     return ZKML_OK;
@@ -374,6 +377,7 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     io.ld_up = c->ld_up;
     io.m = (uint32_t)m;
     io.activation = c->activation;
+    io.act_table = c->activation == 2 ? lin->act_table[0] : c->activation == 5 ? lin->act_table[1] : nullptr;
     const Choice& p = choose(lin->w, io.m, c->x_bits, ctx->num_sms);
     ZK_CUDA(launch_choice(p, lin->w, io, c->workspace, s, true));
     ctx->launches += p.few ? 1 : 2;

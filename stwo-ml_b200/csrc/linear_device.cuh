@@ -37,55 +37,37 @@ __device__ __forceinline__ void activation_digits(const uint4& x, uint32_t (&d)[
     for (int b = 0; b < D; b++) d[b] = p[b];
 }
 
-// SiLU or GELU of the M31 word v with |real| below the saturation bound, canonical.
-// Both are mag * w / (1 + e) in units of 2^-16, with mag = |v|, w = 1 for positive and e for
-// negative v, and e = exp(-a), a = |x| for SiLU and 2 |u| for GELU's inner term u
-// (1 + tanh u = 2 / (1 + exp(-2u))).  e = 2^-k exp(r), |r| <= ln(2) / 2, by the Taylor polynomial
-// of degree 9 (remainder below 2^-37), 1 / (1 + e) by one Newton step from a single-precision
-// estimate (below 2^-43): the result, below 2^21.3, is off by less than 2^-15.  Where it lies
-// within 2^-12 of a half-integer the defining binary64 form decides the rounding.  About 25
-// double-precision operations instead of the 150 and more of exp, tanh and a division.
+// SiLU or GELU of the M31 word v, |v| = mag below act_limit, canonical.  Both functions fall short
+// of max(x, 0) by the same amount on either side of zero: f(x) = x - delta(x) and f(-x) = -delta(x) for
+// x > 0.  delta 2^16 comes from a table of segments, c0 + c1 d + c2 d^2 + c3 d^3 with d the offset from
+// the segment's middle: c0 and c1 d are added as integers in 2^-30 units, the rest, below 4, in single
+// precision.  Over every word below the limit that is off by at most 2^-16.1 (checked against
+// extended precision); where it lies within 2^-14 of a half-integer, 174 words in all, the
+// defining binary64 form decides the rounding.  One 16-byte read and about 25 instructions of full
+// rate; a double-precision exponential took several times as long (512 int8 tokens x 5120 x 13824,
+// whose inputs all bend: 111 us a call).
 // Out of line: copies at every call site made the kernels miss the instruction cache.
-static __device__ __noinline__ uint32_t bent_activation(int tag, uint32_t v, uint32_t mag, bool neg) {
-    const double x = (double)mag * (1.0 / 65536.0);
-    double a = x;
-    if (tag == 2) a = 2.0 * 0.79788456080286535588 * fma(0.044715 * x * x, x, x);  // 2 sqrt(2 / pi) (x + 0.044715 x^3)
-    const int k = __double2int_rn(a * 1.44269504088896340736);  // a / ln 2
-    const double r = fma((double)k, 0.69314718055994530942, -a);
-    double e = 1.0 / 362880.0;
-    e = fma(e, r, 1.0 / 40320.0);
-    e = fma(e, r, 1.0 / 5040.0);
-    e = fma(e, r, 1.0 / 720.0);
-    e = fma(e, r, 1.0 / 120.0);
-    e = fma(e, r, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    e *= __hiloint2double((1023 - k) << 20, 0);  // k < 90
-    const double d = 1.0 + e;
-    const double q0 = (double)__fdividef(1.0f, (float)d);
-    const double q = q0 * fma(-d, q0, 2.0);
-    const double y = (double)mag * (neg ? e * q : q);
-    const double whole = floor(y), rest = y - whole;
-    if (fabs(rest - 0.5) < 1.0 / 4096.0) return red32(act_value(tag, v));
-    const uint32_t n = (uint32_t)whole + (rest >= 0.5 ? 1u : 0u);
-    return neg && n ? P - n : n;
+static __device__ __noinline__ uint32_t bent_activation(const uint8_t* table, int tag, uint32_t v, uint32_t mag, bool neg) {
+    const uint32_t bits = act_segment_bits(tag), half = 1u << (bits - 1);
+    const uint4 s = reinterpret_cast<const uint4*>(table)[mag >> bits];
+    const int d = (int)(mag & (2 * half - 1)) - (int)half;
+    const float e = (float)d, g = fmaf(__uint_as_float(s.w), e, __uint_as_float(s.z)) * (e * e);
+    const int64_t y = (int64_t)((uint64_t)s.x << 13) + (int64_t)(int)s.y * d + ((int64_t)__float2int_rn(g) << 10);
+    const int off = (int)((uint32_t)y & 0x3fffffffu) - 0x20000000;
+    if (abs(off) < 65536) return red32(act_value(tag, v));
+    const uint32_t n = (uint32_t)((y + 0x20000000) >> 30);
+    return !neg ? mag - n : n ? P - n : 0u;
 }
 
-// f(v), canonical.  Where SiLU and GELU equal their argument or round to zero in binary64 the
-// result is taken without evaluating them: for real x >= 37, exp(-x) < 2^-53 and 1 + exp(-x) is
-// 1; for x <= -16, |x| exp(x) 2^16 < 1/2; for |x| >= 8.5, |tanh| of GELU's inner term (above 28)
-// is 1.
-__device__ __forceinline__ uint32_t activate(int tag, uint32_t v) {
+// f(v), canonical.  From act_limit on, delta 2^16 is below 0.12, so SiLU and GELU round to max(x, 0).
+__device__ __forceinline__ uint32_t activate(const uint8_t* table, int tag, uint32_t v) {
     if (tag == 0) return v;
     if (tag == 1) return v <= (P - 1) / 2 ? v : 0u;
     if (tag == 5 || tag == 2) {
         const bool neg = v > (P - 1) / 2;
         const uint32_t mag = neg ? P - v : v;
-        const uint32_t sat = tag == 2 ? (17u << 15) : neg ? (16u << 16) : (37u << 16);
-        if (mag >= sat) return neg ? 0u : v;
-        return bent_activation(tag, v, mag, neg);
+        if (mag >= act_limit(tag)) return neg ? 0u : v;
+        return bent_activation(table, tag, v, mag, neg);
     }
     return red32(act_value(tag, v));
 }
@@ -94,12 +76,15 @@ __device__ __forceinline__ uint32_t activate(int tag, uint32_t v) {
 template <int D>
 constexpr int GROUP = 16 / D;
 
+// x + y mod P for x <= P, y < P.
+__device__ __forceinline__ uint32_t add_mod(uint32_t x, uint32_t y) { return min(x + y, x + y - P); }
+
 // sum_i 256^i acc_i mod P of one token's accumulators.
 template <int D>
 __device__ __forceinline__ uint32_t join_digits(const uint32_t (&r)[16], int t) {
     if (D == 1) {
-        const int v = (int)r[t];
-        return red32(v < 0 ? (uint32_t)(v + 0x7fffffff) : (uint32_t)v);
+        const int v = (int)r[t];  // |v| <= 1023 * 2^21 < P
+        return (uint32_t)(v + ((v >> 31) & 0x7fffffff));
     }
     int64_t s = 0;
 #pragma unroll
@@ -107,19 +92,29 @@ __device__ __forceinline__ uint32_t join_digits(const uint32_t (&r)[16], int t) 
     return canon64((uint64_t)s + ((uint64_t)P << 26));  // |s| < 2^56
 }
 
+__host__ __device__ inline bool io_bends(const LinearIO& io) {
+    return (io.activation == 2 || io.activation == 5) && !io.as_reference;
+}
+
 // f(v) as an output word: canonical, or as the reference's forward pass leaves it (LinearIO::as_reference).
-__device__ __forceinline__ uint32_t activated(const LinearIO& io, uint32_t v) {
+__device__ __forceinline__ uint32_t activated(const LinearIO& io, const uint8_t* table, uint32_t v) {
     if (io.as_reference && io.activation) return act_value(io.activation, v);
-    return activate(io.activation, v);
+    return activate(table, io.activation, v);
 }
 
 // Finishes GROUP tokens of this lane's row: z (without the bias) -> outputs.
 template <int D, bool GATED>
-__device__ __forceinline__ void finish_tokens(const LinearIO& io, uint32_t n, uint32_t nt, uint32_t row, uint32_t tok0,
-                                              uint32_t base, uint32_t (&z)[GROUP<D>]) {
+__device__ __forceinline__ void finish_tokens(const LinearIO& io, const uint8_t* table, uint32_t n, uint32_t nt,
+                                              uint32_t row, uint32_t tok0, uint32_t base, uint32_t (&z)[GROUP<D>]) {
     constexpr int G = GROUP<D>;
+    const bool plain = io.activation <= 1;  // identity and ReLU without a call
+    const bool relu = io.activation == 1;
+    const auto f_of = [&](uint32_t v) {
+        if (plain) return relu && v > (P - 1) / 2 ? 0u : v;
+        return activated(io, table, v);
+    };
 #pragma unroll
-    for (int t = 0; t < G; t++) z[t] = madd(z[t], base);
+    for (int t = 0; t < G; t++) z[t] = add_mod(z[t], base);
     if (GATED) {
         // lane l < 16: gate, lane l + 16: up of the same output; of each token pair one lane
         // finishes the first token and the other the second
@@ -133,25 +128,35 @@ __device__ __forceinline__ void finish_tokens(const LinearIO& io, uint32_t n, ui
             if (f < n && tok < io.m) {
                 if (io.pre) io.pre[(size_t)tok * io.ld_pre + f] = g;
                 if (io.up) io.up[(size_t)tok * io.ld_up + f] = u;
-                io.out[(size_t)tok * io.ld_out + f] = mmul(activated(io, g), u);
+                io.out[(size_t)tok * io.ld_out + f] = mmul(activated(io, table, g), u);
             }
         }
     } else {
         const uint32_t f = nt * LIN_ROWS + row;
         if (f >= n) return;
-        uint32_t res[G], bad = 0;
+        uint32_t* out = io.out + (size_t)tok0 * io.ld_out + f;
+        if (io.pre) {
+            uint32_t* pre = io.pre + (size_t)tok0 * io.ld_pre + f;
 #pragma unroll
-        for (int t = 0; t < G; t++)
-            res[t] = io.residual && tok0 + t < io.m ? __ldcg(io.residual + (size_t)(tok0 + t) * io.ld_res + f) : 0u;
-#pragma unroll
-        for (int t = 0; t < G; t++) {
-            if (tok0 + t >= io.m) continue;
-            if (io.pre) io.pre[(size_t)(tok0 + t) * io.ld_pre + f] = z[t];
-            bad |= res[t] >> 31;
-            const uint32_t y = activated(io, z[t]);
-            io.out[(size_t)(tok0 + t) * io.ld_out + f] = io.residual ? madd(y, red32(res[t])) : y;
+            for (int t = 0; t < G; t++, pre += io.ld_pre)
+                if (tok0 + t < io.m) *pre = z[t];
         }
-        if (bad) atomicOr(io.status, LIN_BAD_VALUE);
+        if (io.residual) {
+            uint32_t res[G], bad = 0;
+            const uint32_t* r = io.residual + (size_t)tok0 * io.ld_res + f;
+#pragma unroll
+            for (int t = 0; t < G; t++, r += io.ld_res) res[t] = tok0 + t < io.m ? __ldcg(r) : 0u;
+#pragma unroll
+            for (int t = 0; t < G; t++, out += io.ld_out) {
+                bad |= res[t] >> 31;
+                if (tok0 + t < io.m) *out = add_mod(f_of(z[t]), red32(res[t]));
+            }
+            if (bad) atomicOr(io.status, LIN_BAD_VALUE);
+        } else {
+#pragma unroll
+            for (int t = 0; t < G; t++, out += io.ld_out)
+                if (tok0 + t < io.m) *out = f_of(z[t]);
+        }
     }
 }
 

@@ -24,6 +24,8 @@ namespace zk {
 
 namespace {
 
+__device__ __align__(16) uint8_t act_tables[act_table_bytes(2) + act_table_bytes(5)];  // GELU, SiLU
+
 // Epilogue warps: four to each quarter of the accumulators' rows, taking every fourth token group.
 // One warp a quarter left each scheduler a single chain of dependent instructions and bound most
 // calls by it (64 tokens x 5120 x 13824: 58 us with 4 warps).
@@ -257,7 +259,7 @@ __device__ __forceinline__ bool all_of_epilogue(bool ok) {
 template <int D, bool GATED>
 __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constant__ KernelArgs a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * 16 + 5];
+    __shared__ __align__(8) uint64_t bars[2 * 16 + 6];
     __shared__ uint32_t tmem_base_s, last_s;
     __shared__ volatile uint32_t quit_s;
     constexpr int G = GROUP<D>;
@@ -265,7 +267,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
     const uint32_t n_cols = D * a.tokens, b_bytes = n_cols * LIN_KB, stage_bytes = LIN_TILE_BYTES + b_bytes;
     const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
     const uint32_t full = smem_addr(bars), empty = full + 8 * 16, acc_full = empty + 8 * 16, acc_empty = acc_full + 16;
-    const uint32_t drained = acc_empty + 16;
+    const uint32_t drained = acc_empty + 16, table_full = drained + 8;
+    const bool bends = io_bends(a.io);  // the activation takes its table, kept behind the stages
+    const uint32_t table_at = smem0 + a.stages * stage_bytes, table_bytes = act_table_bytes(a.io.activation);
     uint32_t cols = 32;
     while (cols < 2 * n_cols) cols <<= 1;
     if (threadIdx.x == 0) {
@@ -279,6 +283,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
             mbar_init(acc_empty + 8 * i, EPI_THREADS);
         }
         mbar_init(drained, 1);
+        mbar_init(table_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();  // the block barriers want whole warps
@@ -325,6 +330,10 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                 bulk_load(smem0 + i * stage_bytes, wp, LIN_TILE_BYTES, full + 8 * i);
                 issued++;
             }
+            if (bends) {
+                mbar_expect_tx(table_full, table_bytes);
+                bulk_load(table_at, a.io.act_table, table_bytes, table_full);
+            }
             grid_dependency_wait();
 #pragma unroll
             for (uint32_t i = 0; i < 16; i++)
@@ -342,6 +351,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
             if (quit_s) {  // copies in flight land before the block ends
                 atomicOr(a.io.status, LIN_TIMEOUT);
                 volatile uint32_t never = 0;
+                if (bends) mbar_wait(table_full, 0, &never);
                 for (uint32_t i = 0; i < min(issued, a.stages); i++) {
                     const uint32_t u = issued - 1 - i;
                     mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never);
@@ -391,11 +401,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
         sch.init(a);
         Segment s{};
         uint32_t seg = 0;
+        const bool have_table = !bends || mbar_wait(table_full, 0, &quit_s);
+        const uint8_t* table = smem_raw + (table_at - smem_addr(smem_raw));
         uint32_t* const my_slots = a.slots + (size_t)blockIdx.x * a.slots_per_cta * a.tokens * LIN_ROWS;
         while (sch.next(s)) {
             const uint32_t buf = seg & 1, use = seg >> 1;
             seg++;
-            if (!all_of_epilogue(mbar_wait(acc_full + 8 * buf, use & 1, &quit_s))) break;
+            if (!all_of_epilogue(have_table && mbar_wait(acc_full + 8 * buf, use & 1, &quit_s))) break;
             tc_fence_after();
             uint32_t mt, nt;
             tile_at(a, s.tile, mt, nt);
@@ -425,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                     for (int t = 0; t < G; t++) z[t] = madd(z[t], slot[(size_t)(t0 + t) * LIN_ROWS]);
                 }
                 if (direct) {
-                    finish_tokens<D, GATED>(a.io, a.w.n, nt, row, mt * a.tokens + t0, base, z);
+                    finish_tokens<D, GATED>(a.io, table, a.w.n, nt, row, mt * a.tokens + t0, base, z);
                 } else {
 #pragma unroll
                     for (int t = 0; t < G; t++) slot[(size_t)(t0 + t) * LIN_ROWS] = z[t];
@@ -473,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                     }
 #pragma unroll
                     for (int t = 0; t < G; t++) z[t] = canon64(sum[t]);
-                    finish_tokens<D, GATED>(a.io, a.w.n, nt, row, mt * a.tokens + t0, base, z);
+                    finish_tokens<D, GATED>(a.io, table, a.w.n, nt, row, mt * a.tokens + t0, base, z);
                 }
             }
             asm volatile("bar.sync 1, %0;" ::"n"(EPI_THREADS) : "memory");  // last_s is read before it is written again
@@ -485,7 +497,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
     if (warp == 2) tmem_free(tmem, cols);
 }
 
-constexpr uint32_t SMEM_MAX = 220 * 1024;
+constexpr uint32_t SMEM_MAX = 225 * 1024;
+constexpr uint32_t STAGES_MAX = SMEM_MAX - 1024 - ACT_TABLE_MAX;  // bytes of all stages
 
 template <int D, bool GATED>
 cudaError_t configure_one() {
@@ -500,7 +513,9 @@ cudaError_t launch_all(const KernelArgs& a, const LinearPlan& p, uint8_t* digits
     cudaError_t e = cudaLaunchKernelEx(&d.cfg, linear_digits_kernel<D>, a.io.x, a.io.ldx, a.io.m, w.k, w.k_tiles,
                                        p.tokens, digits, a.counters, p.sk_tiles, a.io.status);
     if (e != cudaSuccess) return e;
-    const Launch l(dim3(p.ctas), THREADS, p.stages * (LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB) + 1024, s, overlap);
+    const uint32_t smem = 1024 + p.stages * (LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB) +
+                          (io_bends(a.io) ? ACT_TABLE_MAX : 0);
+    const Launch l(dim3(p.ctas), THREADS, smem, s, overlap);
     return w.gated ? cudaLaunchKernelEx(&l.cfg, linear_kernel<D, true>, a)
                    : cudaLaunchKernelEx(&l.cfg, linear_kernel<D, false>, a);
 }
@@ -576,7 +591,7 @@ LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_s
     }
     LinearPlan& p = best;
     const uint32_t stage = LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB;
-    p.stages = std::min(16u, (SMEM_MAX - 1024) / stage);
+    p.stages = std::min(16u, STAGES_MAX / stage);
     p.slots = w.planes > 1 || w.k_tiles > KSEG ? 3 : p.sk_tiles ? 2 : 0;
     auto up = [](size_t v) { return (v + 1023) / 1024 * 1024; };
     p.digits_off = up((size_t)p.sk_tiles * 4);
@@ -585,8 +600,20 @@ LinearPlan linear_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_s
     return p;
 }
 
+cudaError_t linear_act_table(int tag, const uint8_t** out) {
+    *out = nullptr;
+    if (tag != 2 && tag != 5) return cudaSuccess;
+    void* p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, act_tables);
+    if (e == cudaSuccess) *out = static_cast<const uint8_t*>(p) + (tag == 5 ? act_table_bytes(2) : 0);
+    return e;
+}
+
 cudaError_t linear_configure() {
-    cudaError_t e = configure_one<1, false>();
+    cudaError_t e = cudaMemcpyToSymbol(act_tables, act_segment_table(2), act_table_bytes(2), 0);
+    if (e == cudaSuccess)
+        e = cudaMemcpyToSymbol(act_tables, act_segment_table(5), act_table_bytes(5), act_table_bytes(2));
+    if (e == cudaSuccess) e = configure_one<1, false>();
     if (e == cudaSuccess) e = configure_one<2, false>();
     if (e == cudaSuccess) e = configure_one<4, false>();
     if (e == cudaSuccess) e = configure_one<1, true>();

@@ -260,14 +260,14 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
                 }
 #pragma unroll
                 for (int t = 0; t < G; t++) z[h][t] = canon64(sum[t]);
-                finish_tokens<D, GATED>(a.io, a.w.n, nt, row, h * G, base, z[h]);
+                finish_tokens<D, GATED>(a.io, a.io.act_table, a.w.n, nt, row, h * G, base, z[h]);
             }
         }
     } else if (finisher && ok) {
 #pragma unroll
         for (uint32_t h = 0; h < GROUPS; h++) {
             if (h * G >= a.io.m) break;
-            finish_tokens<D, GATED>(a.io, a.w.n, nt, row, h * G, base, z[h]);
+            finish_tokens<D, GATED>(a.io, a.io.act_table, a.w.n, nt, row, h * G, base, z[h]);
         }
     }
     __syncwarp();
