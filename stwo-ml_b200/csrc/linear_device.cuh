@@ -37,39 +37,54 @@ __device__ __forceinline__ void activation_digits(const uint4& x, uint32_t (&d)[
     for (int b = 0; b < D; b++) d[b] = p[b];
 }
 
-// SiLU or GELU of the M31 word v, |v| = mag below act_limit, canonical.  Both functions fall short
+// SiLU or GELU of M31 words, canonical, with mag = |v|.  Both functions fall short
 // of max(x, 0) by the same amount on either side of zero: f(x) = x - delta(x) and f(-x) = -delta(x) for
 // x > 0.  delta 2^16 comes from a table of segments, c0 + c1 d + c2 d^2 + c3 d^3 with d the offset from
 // the segment's middle: c0 and c1 d are added as integers in 2^-30 units, the rest, below 4, in single
 // precision.  Over every word below the limit that is off by at most 2^-16.1 (checked against
 // extended precision); where it lies within 2^-14 of a half-integer, 174 words in all, the
 // defining binary64 form decides the rounding.  One 16-byte read and about 25 instructions of full
-// rate; a double-precision exponential took several times as long (512 int8 tokens x 5120 x 13824,
-// whose inputs all bend: 111 us a call).
-// Out of line: copies at every call site made the kernels miss the instruction cache.
-static __device__ __noinline__ uint32_t bent_activation(const uint8_t* table, int tag, uint32_t v, uint32_t mag, bool neg) {
-    const uint32_t bits = act_segment_bits(tag), half = 1u << (bits - 1);
-    const uint4 s = reinterpret_cast<const uint4*>(table)[mag >> bits];
-    const int d = (int)(mag & (2 * half - 1)) - (int)half;
-    const float e = (float)d, g = fmaf(__uint_as_float(s.w), e, __uint_as_float(s.z)) * (e * e);
-    const int64_t y = (int64_t)((uint64_t)s.x << 13) + (int64_t)(int)s.y * d + ((int64_t)__float2int_rn(g) << 10);
-    const int off = (int)((uint32_t)y & 0x3fffffffu) - 0x20000000;
-    if (abs(off) < 65536) return red32(act_value(tag, v));
-    const uint32_t n = (uint32_t)((y + 0x20000000) >> 30);
-    return !neg ? mag - n : n ? P - n : 0u;
-}
-
-// f(v), canonical.  From act_limit on, delta 2^16 is below 0.12, so SiLU and GELU round to max(x, 0).
-__device__ __forceinline__ uint32_t activate(const uint8_t* table, int tag, uint32_t v) {
-    if (tag == 0) return v;
-    if (tag == 1) return v <= (P - 1) / 2 ? v : 0u;
-    if (tag == 5 || tag == 2) {
-        const bool neg = v > (P - 1) / 2;
-        const uint32_t mag = neg ? P - v : v;
-        if (mag >= act_limit(tag)) return neg ? 0u : v;
-        return bent_activation(table, tag, v, mag, neg);
+// rate a value (512 int8 tokens x 5120 x 13824, whose inputs all bend: 65 us a call, 46 us with ReLU;
+// 110 us with a double-precision exponential).
+// Several values a call, so that their reads and sums overlap; from act_limit on, delta 2^16 is below
+// 0.12 and f rounds to max(x, 0).  Out of line: copies at every call site made the kernels miss the
+// instruction cache.
+template <int N>
+struct Words {
+    uint32_t v[N];
+};
+template <int N>
+static __device__ __noinline__ Words<N> bent_activation(const uint8_t* table, int tag, Words<N> x) {
+    const uint32_t bits = act_segment_bits(tag), half = 1u << (bits - 1), limit = act_limit(tag);
+    uint32_t mag[N], n[N];
+    uint4 s[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        mag[i] = min(x.v[i], P - x.v[i]);
+        s[i] = reinterpret_cast<const uint4*>(table)[min(mag[i], limit - 1) >> bits];
     }
-    return red32(act_value(tag, v));
+    bool unsure = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int d = (int)(mag[i] & (2 * half - 1)) - (int)half;
+        const float e = (float)d, g = fmaf(__uint_as_float(s[i].w), e, __uint_as_float(s[i].z)) * (e * e);
+        const int64_t t =
+            (int64_t)((uint64_t)s[i].x << 13) + (int64_t)(int)s[i].y * d + ((int64_t)__float2int_rn(g) << 10);
+        const int off = (int)((uint32_t)t & 0x3fffffffu) - 0x20000000;
+        n[i] = mag[i] < limit ? (uint32_t)((t + 0x20000000) >> 30) : 0u;
+        unsure |= abs(off) < 65536 && mag[i] < limit;
+    }
+    Words<N> y;
+#pragma unroll
+    for (int i = 0; i < N; i++) {  // delta: off a positive value, and what a negative one comes to below zero
+        const uint32_t r = (x.v[i] > (P - 1) / 2 ? 0u : x.v[i]) + P - n[i];
+        y.v[i] = r >= P ? r - P : r;
+    }
+    if (unsure) {
+#pragma unroll
+        for (int i = 0; i < N; i++) y.v[i] = red32(act_value(tag, x.v[i]));
+    }
+    return y;
 }
 
 // Tokens handled together: their digits are 16 accumulator columns.
@@ -96,10 +111,39 @@ __host__ __device__ inline bool io_bends(const LinearIO& io) {
     return (io.activation == 2 || io.activation == 5) && !io.as_reference;
 }
 
-// f(v) as an output word: canonical, or as the reference's forward pass leaves it (LinearIO::as_reference).
-__device__ __forceinline__ uint32_t activated(const LinearIO& io, const uint8_t* table, uint32_t v) {
-    if (io.as_reference && io.activation) return act_value(io.activation, v);
-    return activate(table, io.activation, v);
+// y = f(y): canonical, or as the reference's forward pass leaves it (LinearIO::as_reference).
+template <int N>  // 1 or a multiple of 4
+__device__ __forceinline__ void activate(const LinearIO& io, const uint8_t* table, uint32_t (&y)[N]) {
+    constexpr int CHUNK = N < 4 ? N : 4;
+    if (io.activation == 0) return;
+    if (io.activation == 1) {
+#pragma unroll
+        for (int t = 0; t < N; t++) y[t] = y[t] > (P - 1) / 2 ? 0u : y[t];
+    } else if (io_bends(io)) {
+#pragma unroll
+        for (int t = 0; t < N; t += CHUNK) {
+            uint32_t least = P;
+#pragma unroll
+            for (int i = 0; i < CHUNK; i++) least = min(least, min(y[t + i], P - y[t + i]));
+            if (least < act_limit(io.activation)) {
+                Words<CHUNK> q;
+#pragma unroll
+                for (int i = 0; i < CHUNK; i++) q.v[i] = y[t + i];
+                q = bent_activation(table, io.activation, q);
+#pragma unroll
+                for (int i = 0; i < CHUNK; i++) y[t + i] = q.v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < CHUNK; i++) y[t + i] = y[t + i] > (P - 1) / 2 ? 0u : y[t + i];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < N; t++) {
+            const uint32_t v = act_value(io.activation, y[t]);
+            y[t] = io.as_reference ? v : red32(v);
+        }
+    }
 }
 
 // Finishes GROUP tokens of this lane's row: z (without the bias) -> outputs.
@@ -107,12 +151,6 @@ template <int D, bool GATED>
 __device__ __forceinline__ void finish_tokens(const LinearIO& io, const uint8_t* table, uint32_t n, uint32_t nt,
                                               uint32_t row, uint32_t tok0, uint32_t base, uint32_t (&z)[GROUP<D>]) {
     constexpr int G = GROUP<D>;
-    const bool plain = io.activation <= 1;  // identity and ReLU without a call
-    const bool relu = io.activation == 1;
-    const auto f_of = [&](uint32_t v) {
-        if (plain) return relu && v > (P - 1) / 2 ? 0u : v;
-        return activated(io, table, v);
-    };
 #pragma unroll
     for (int t = 0; t < G; t++) z[t] = add_mod(z[t], base);
     if (GATED) {
@@ -120,43 +158,62 @@ __device__ __forceinline__ void finish_tokens(const LinearIO& io, const uint8_t*
         // finishes the first token and the other the second
         const bool up_lane = (row & 16) != 0;
         const uint32_t f = nt * 64 + (row >> 5) * 16 + (row & 15);
+        // pairs by four where a group has as many, so that their activations overlap
+        constexpr int PAIRS = G >= 8 ? 4 : 1;
 #pragma unroll
-        for (int t = 0; t < G; t += 2) {
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, up_lane ? z[t] : z[t + 1], 16);
-            const uint32_t g = up_lane ? got : z[t], u = up_lane ? z[t + 1] : got;
+        for (int t = 0; t < G; t += 2 * PAIRS) {
+            uint32_t y[PAIRS], u[PAIRS];
+#pragma unroll
+            for (int i = 0; i < PAIRS; i++) {
+                const uint32_t a = z[t + 2 * i], b = z[t + 2 * i + 1];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up_lane ? a : b, 16);
+                y[i] = up_lane ? got : a;
+                u[i] = up_lane ? b : got;
+            }
             const uint32_t tok = tok0 + t + (up_lane ? 1 : 0);
             if (f < n && tok < io.m) {
-                if (io.pre) io.pre[(size_t)tok * io.ld_pre + f] = g;
-                if (io.up) io.up[(size_t)tok * io.ld_up + f] = u;
-                io.out[(size_t)tok * io.ld_out + f] = mmul(activated(io, table, g), u);
+                if (io.pre) {
+#pragma unroll
+                    for (int i = 0; i < PAIRS; i++)
+                        if (tok + 2 * i < io.m) io.pre[(size_t)(tok + 2 * i) * io.ld_pre + f] = y[i];
+                }
+                if (io.up) {
+#pragma unroll
+                    for (int i = 0; i < PAIRS; i++)
+                        if (tok + 2 * i < io.m) io.up[(size_t)(tok + 2 * i) * io.ld_up + f] = u[i];
+                }
+                activate(io, table, y);
+#pragma unroll
+                for (int i = 0; i < PAIRS; i++)
+                    if (tok + 2 * i < io.m) io.out[(size_t)(tok + 2 * i) * io.ld_out + f] = mmul(y[i], u[i]);
             }
         }
     } else {
         const uint32_t f = nt * LIN_ROWS + row;
         if (f >= n) return;
-        uint32_t* out = io.out + (size_t)tok0 * io.ld_out + f;
         if (io.pre) {
             uint32_t* pre = io.pre + (size_t)tok0 * io.ld_pre + f;
 #pragma unroll
             for (int t = 0; t < G; t++, pre += io.ld_pre)
                 if (tok0 + t < io.m) *pre = z[t];
         }
+        activate(io, table, z);
         if (io.residual) {
             uint32_t res[G], bad = 0;
             const uint32_t* r = io.residual + (size_t)tok0 * io.ld_res + f;
 #pragma unroll
             for (int t = 0; t < G; t++, r += io.ld_res) res[t] = tok0 + t < io.m ? __ldcg(r) : 0u;
 #pragma unroll
-            for (int t = 0; t < G; t++, out += io.ld_out) {
+            for (int t = 0; t < G; t++) {
                 bad |= res[t] >> 31;
-                if (tok0 + t < io.m) *out = add_mod(f_of(z[t]), red32(res[t]));
+                z[t] = add_mod(z[t], red32(res[t]));
             }
             if (bad) atomicOr(io.status, LIN_BAD_VALUE);
-        } else {
-#pragma unroll
-            for (int t = 0; t < G; t++, out += io.ld_out)
-                if (tok0 + t < io.m) *out = f_of(z[t]);
         }
+        uint32_t* out = io.out + (size_t)tok0 * io.ld_out + f;
+#pragma unroll
+        for (int t = 0; t < G; t++, out += io.ld_out)
+            if (tok0 + t < io.m) *out = z[t];
     }
 }
 
