@@ -12,6 +12,20 @@ namespace zk {
 
 constexpr uint32_t KSEG = 1023;  // K tiles per 32-bit accumulation: 1023 * 128 * 2^14 < 2^31
 
+// Activations are read by these: cached in L1 (neighbouring lanes and loads share sectors), but not as
+// data that stays constant while the kernel runs, since a programmatic dependent starts before the
+// work that writes them is done.
+__device__ __forceinline__ uint32_t load_word(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint4 load_words(const uint32_t* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // The four balanced byte digits of v (|v| < 2^31 - 2^23), byte i holding the digit of 256^i in
 // [-128, 127]: adding 128 to every digit makes them the plain base-256 digits of v + 0x80808080.
 __device__ __forceinline__ uint32_t balanced_digits(int v) { return ((uint32_t)v + 0x80808080u) ^ 0x80808080u; }

@@ -123,7 +123,7 @@ __global__ void linear_base_kernel(const unsigned long long* __restrict__ sums, 
 // i x tokens + t the digit i of token t.  A block takes 32 tokens of a tile (all, if fewer), a
 // thread 16 K of one token.  Block 0 also zeroes the counters of the cut tiles.
 template <int D>
-__global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* __restrict__ x, size_t ldx, uint32_t m,
+__global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* x, size_t ldx, uint32_t m,
                                                             uint32_t k, uint32_t k_tiles, uint32_t tokens,
                                                             uint8_t* __restrict__ out, uint32_t* __restrict__ counters,
                                                             uint32_t n_counters, uint32_t* __restrict__ status) {
@@ -138,13 +138,13 @@ __global__ void __launch_bounds__(256) linear_digits_kernel(const uint32_t* __re
     const uint32_t t = blockIdx.y * 32 + threadIdx.x / 8, c = threadIdx.x % 8;
     if (t < tokens) {
         const uint32_t row = mt * tokens + t, k0 = kt * LIN_KB + 16 * c;
-        uint4 v[4];  // from L2: earlier work may have written x since this grid's blocks started
+        uint4 v[4];
         const uint32_t* src = x + (size_t)row * ldx + k0;
         if (row < m && vec && k0 + 16 <= k) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = __ldcg(reinterpret_cast<const uint4*>(src) + i);
+            for (int i = 0; i < 4; i++) v[i] = load_words(src + 4 * i);
         } else {
-            const auto at = [&](uint32_t i) { return row < m && k0 + i < k ? __ldcg(src + i) : 0u; };
+            const auto at = [&](uint32_t i) { return row < m && k0 + i < k ? load_word(src + i) : 0u; };
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) v[i] = make_uint4(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));
         }

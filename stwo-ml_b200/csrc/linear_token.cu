@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         const uint32_t maker = warp - 2, slice = maker % a.slices, groups = min(MAKERS / a.slices, a.stages);
         const bool vec = (a.io.ldx % 4 == 0) && ((reinterpret_cast<uintptr_t>(a.io.x) & 15) == 0);
         uint32_t bad = 0;
-        const auto load = [&](uint4(&v)[2], uint32_t u) {  // from L2: earlier work may have written x since this block started
+        const auto load = [&](uint4(&v)[2], uint32_t u) {
             uint32_t plane, kt;
             tile_of(u, plane, kt);
             const uint32_t k0 = kt * LIN_KB + 4 * lane;
@@ -154,12 +154,12 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
                 if (t >= a.io.m) continue;
                 const uint32_t* src = a.io.x + (size_t)t * a.io.ldx + k0;
                 if (vec && k0 + 4 <= a.w.k) {
-                    v[i] = __ldcg(reinterpret_cast<const uint4*>(src));
+                    v[i] = load_words(src);
                 } else {
-                    if (k0 < a.w.k) v[i].x = __ldcg(src);
-                    if (k0 + 1 < a.w.k) v[i].y = __ldcg(src + 1);
-                    if (k0 + 2 < a.w.k) v[i].z = __ldcg(src + 2);
-                    if (k0 + 3 < a.w.k) v[i].w = __ldcg(src + 3);
+                    if (k0 < a.w.k) v[i].x = load_word(src);
+                    if (k0 + 1 < a.w.k) v[i].y = load_word(src + 1);
+                    if (k0 + 2 < a.w.k) v[i].z = load_word(src + 2);
+                    if (k0 + 3 < a.w.k) v[i].w = load_word(src + 3);
                 }
             }
         };
