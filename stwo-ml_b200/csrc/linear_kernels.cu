@@ -533,7 +533,7 @@ void launch_linear_base(const unsigned long long* sums, const uint32_t* bias, co
 }
 
 // Clocks of a split: a model with rates fitted to 916 measured splits of 33 calls (m 9 to 2048, K 300
-// to 13824; the split it picks takes 2 % longer than the fastest on average, 13 % at worst).  A block
+// to 13824; the split it picks takes 4 % longer than the fastest on average, 16 % at worst).  A block
 // multiplies 128 rows x N columns x 128 K in 2 N clocks and takes in 46 bytes a clock, all blocks
 // together 5500; a token of a tile costs 30 clocks to finish, under the next tile's products
 // except for the last tile; cutting tiles costs a round through memory for the parts, 5200 clocks
