@@ -451,7 +451,8 @@ int zkml_linear_workspace(const zkml_linear *lin, size_t m, int x_bits, size_t *
  * the next zkml_linear_check reports it. */
 int zkml_linear_forward(zkml_linear *lin, const zkml_linear_call *call);
 /* Waits for `stream` (NULL: the context's stream) and reports, once, whether a call since the
- * last check met such a value. */
+ * last check met such a value (ZKML_ERR_INVALID_ARG), or gave up on a wait inside its kernels and left
+ * outputs unwritten (ZKML_ERR_TIMEOUT: two seconds without progress). */
 int zkml_linear_check(zkml_linear *lin, void *stream);
 
 /* ---- Stepwise product sumcheck (multi-GPU building block) -------------------
@@ -540,6 +541,14 @@ int zkml_prove_product_sharded(zkml_ctx *ctx, const uint32_t *a_local, const uin
  * never posted; *status_out = 1 when its wait ran out and it flagged the
  * timeout instead of hanging.  Takes a few seconds; no GPU fault is involved. */
 int zkml_selftest_wait_timeout(zkml_ctx *ctx, uint32_t *status_out);
+
+/* Self-test of the forward kernels' bounded waits: the call of zkml_linear_forward (weights that are not
+ * gated, x_bits 31) with a limit of limit_ms (1 to 1000) on every wait, and one signal of one block
+ * withheld, so that a wait of that block runs out: 1 its accumulators' completion, 2 a copy of weights, 3
+ * the copy of the activation table (SiLU or GELU, a call with a workspace), 4 a tile of activations
+ * (a call without one).  The kernel gives up and ends; that block's outputs are not written, and
+ * zkml_linear_check returns ZKML_ERR_TIMEOUT.  No GPU fault is involved. */
+int zkml_selftest_linear_wait(zkml_linear *lin, const zkml_linear_call *call, int withhold, uint32_t limit_ms);
 
 /* ---- Allocation-free restriction ------------------------------------------- */
 

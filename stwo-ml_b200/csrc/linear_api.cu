@@ -321,7 +321,8 @@ int zkml_linear_workspace(const zkml_linear* lin, size_t m, int x_bits, size_t* 
     return ZKML_OK;
 }
 
-int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
+// The call of zkml_linear_forward; withhold and wait_ns as in LinearIO.
+static int forward(zkml_linear* lin, const zkml_linear_call* c, int withhold, uint64_t wait_ns) {
     if (!lin || !c || !c->x || !c->out) return set_error(ZKML_ERR_INVALID_ARG, "NULL argument");
     size_t need = 0;
     int rc = zkml_linear_workspace(lin, c->m, c->x_bits, &need);
@@ -378,10 +379,24 @@ int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* c) {
     io.m = (uint32_t)m;
     io.activation = c->activation;
     io.act_table = c->activation == 2 ? lin->act_table[0] : c->activation == 5 ? lin->act_table[1] : nullptr;
+    if (wait_ns) io.wait_ns = wait_ns;
+    io.withhold = withhold;
     const Choice& p = choose(lin->w, io.m, c->x_bits, ctx->num_sms);
+    if ((withhold == LIN_WITHHOLD_TABLE && (p.few || !io.act_table)) || (withhold == LIN_WITHHOLD_DIGITS && !p.few))
+        return set_error(ZKML_ERR_INVALID_ARG, "the kernel of this call has no such wait");
     ZK_CUDA(launch_choice(p, lin->w, io, c->workspace, s, true));
     ctx->launches += p.few ? 1 : 2;
     return ZKML_OK;
+}
+
+int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* call) { return forward(lin, call, 0, 0); }
+
+int zkml_selftest_linear_wait(zkml_linear* lin, const zkml_linear_call* call, int withhold, uint32_t limit_ms) {
+    if (!lin || !call) return set_error(ZKML_ERR_INVALID_ARG, "NULL argument");
+    if (withhold < LIN_WITHHOLD_DONE || withhold > LIN_WITHHOLD_DIGITS || limit_ms == 0 || limit_ms > 1000 ||
+        lin->w.gated || call->x_bits != 31)
+        return set_error(ZKML_ERR_INVALID_ARG, "self-test: withhold 1 to 4, 1 to 1000 ms, plain weights, x_bits 31");
+    return forward(lin, call, withhold, limit_ms * 1000000ull);
 }
 
 int zkml_linear_check(zkml_linear* lin, void* stream) {

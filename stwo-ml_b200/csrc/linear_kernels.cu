@@ -256,13 +256,15 @@ __device__ __forceinline__ bool all_of_epilogue(bool ok) {
     return r != 0;
 }
 
-template <int D, bool GATED>
+// SELFTEST: with LinearIO::withhold (the instantiation of zkml_selftest_linear_wait alone).
+template <int D, bool GATED, bool SELFTEST = false>
 __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constant__ KernelArgs a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * 16 + 6];
-    __shared__ uint32_t tmem_base_s, last_s;
+    __shared__ uint32_t tmem_base_s, last_s, issued_s;
     __shared__ volatile uint32_t quit_s;
     constexpr int G = GROUP<D>;
+    const int withhold = SELFTEST && blockIdx.x == 0 ? a.io.withhold : 0;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t n_cols = D * a.tokens, b_bytes = n_cols * LIN_KB, stage_bytes = LIN_TILE_BYTES + b_bytes;
     const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
@@ -325,12 +327,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
 #pragma unroll
             for (uint32_t i = 0; i < 16; i++) {
                 if (i >= a.stages || !(more = advance())) break;
+                if (SELFTEST && withhold == LIN_WITHHOLD_COPY && i == 0) break;
                 first_x[i] = xp;
                 mbar_expect_tx(full + 8 * i, stage_bytes);
                 bulk_load(smem0 + i * stage_bytes, wp, LIN_TILE_BYTES, full + 8 * i);
                 issued++;
             }
-            if (bends) {
+            if (bends && !(SELFTEST && withhold == LIN_WITHHOLD_TABLE)) {
                 mbar_expect_tx(table_full, table_bytes);
                 bulk_load(table_at, a.io.act_table, table_bytes, table_full);
             }
@@ -341,22 +344,14 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                     bulk_load(smem0 + i * stage_bytes + LIN_TILE_BYTES, first_x[i], b_bytes, full + 8 * i);
             uint32_t st = 0, phase = 0;
             while (more && issued >= a.stages && advance()) {
-                if (!mbar_wait(empty + 8 * st, phase, &quit_s)) break;
+                if (!mbar_wait(empty + 8 * st, phase, &quit_s, a.io.wait_ns)) break;
                 mbar_expect_tx(full + 8 * st, stage_bytes);
                 bulk_load(smem0 + st * stage_bytes, wp, LIN_TILE_BYTES, full + 8 * st);
                 bulk_load(smem0 + st * stage_bytes + LIN_TILE_BYTES, xp, b_bytes, full + 8 * st);
                 issued++;
                 if (++st == a.stages) st = 0, phase ^= 1;
             }
-            if (quit_s) {  // copies in flight land before the block ends
-                atomicOr(a.io.status, LIN_TIMEOUT);
-                volatile uint32_t never = 0;
-                if (bends) mbar_wait(table_full, 0, &never);
-                for (uint32_t i = 0; i < min(issued, a.stages); i++) {
-                    const uint32_t u = issued - 1 - i;
-                    mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never);
-                }
-            }
+            issued_s = issued;
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -370,11 +365,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
             bool ok = true;
             while (ok && sch.next(s)) {
                 const uint32_t buf = seg & 1, use = seg >> 1;
-                ok = mbar_wait(acc_empty + 8 * buf, (use & 1) ^ 1, &quit_s);
+                ok = mbar_wait(acc_empty + 8 * buf, (use & 1) ^ 1, &quit_s, a.io.wait_ns);
                 tc_fence_after();
                 const uint32_t d = tmem + buf * (cols / 2);
                 for (uint32_t u = 0; ok && u < s.len; u++) {
-                    if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s))) break;
+                    if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s, a.io.wait_ns))) break;
                     tc_fence_after();
                     const uint64_t da = tc_desc_k128(smem0 + st * stage_bytes);
                     const uint64_t db = tc_desc_k128(smem0 + st * stage_bytes + LIN_TILE_BYTES);
@@ -383,14 +378,8 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                     tc_commit(empty + 8 * st);
                     if (++st == a.stages) st = 0, phase ^= 1;
                 }
-                if (ok) tc_commit(acc_full + 8 * buf);
+                if (ok && !(SELFTEST && withhold == LIN_WITHHOLD_DONE && seg == 0)) tc_commit(acc_full + 8 * buf);
                 seg++;
-            }
-            if (!ok) {  // products in flight end before the block does
-                atomicOr(a.io.status, LIN_TIMEOUT);
-                volatile uint32_t never = 0;
-                tc_commit(drained);
-                mbar_wait(drained, 0, &never);
             }
         }
     } else {
@@ -401,13 +390,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
         sch.init(a);
         Segment s{};
         uint32_t seg = 0;
-        const bool have_table = !bends || mbar_wait(table_full, 0, &quit_s);
+        const bool have_table = !bends || mbar_wait(table_full, 0, &quit_s, a.io.wait_ns);
         const uint8_t* table = smem_raw + (table_at - smem_addr(smem_raw));
         uint32_t* const my_slots = a.slots + (size_t)blockIdx.x * a.slots_per_cta * a.tokens * LIN_ROWS;
         while (sch.next(s)) {
             const uint32_t buf = seg & 1, use = seg >> 1;
             seg++;
-            if (!all_of_epilogue(have_table && mbar_wait(acc_full + 8 * buf, use & 1, &quit_s))) break;
+            if (!all_of_epilogue(have_table && mbar_wait(acc_full + 8 * buf, use & 1, &quit_s, a.io.wait_ns))) break;
             tc_fence_after();
             uint32_t mt, nt;
             tile_at(a, s.tile, mt, nt);
@@ -494,15 +483,33 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (quit_s) {
+        // some role's wait ran out (all roles are done now): reported, and the copies and products still in
+        // flight end before the tensor memory and the block do
+        volatile uint32_t never = 0;
+        if (threadIdx.x == 0) {
+            atomicOr(a.io.status, LIN_TIMEOUT);
+            for (uint32_t i = 0; i < min(issued_s, a.stages); i++) {
+                const uint32_t u = issued_s - 1 - i;
+                mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never, a.io.wait_ns);
+            }
+            if (bends) mbar_wait(table_full, 0, &never, a.io.wait_ns);
+        } else if (threadIdx.x == 32) {  // the products' issuer
+            tc_commit(drained);
+            mbar_wait(drained, 0, &never, a.io.wait_ns);
+        }
+        __syncwarp();
+        __syncthreads();
+    }
     if (warp == 2) tmem_free(tmem, cols);
 }
 
 constexpr uint32_t SMEM_MAX = 225 * 1024;
 constexpr uint32_t STAGES_MAX = SMEM_MAX - 1024 - ACT_TABLE_MAX;  // bytes of all stages
 
-template <int D, bool GATED>
+template <int D, bool GATED, bool SELFTEST = false>
 cudaError_t configure_one() {
-    return cudaFuncSetAttribute(linear_kernel<D, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+    return cudaFuncSetAttribute(linear_kernel<D, GATED, SELFTEST>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
 }
 
 template <int D>
@@ -516,6 +523,7 @@ cudaError_t launch_all(const KernelArgs& a, const LinearPlan& p, uint8_t* digits
     const uint32_t smem = 1024 + p.stages * (LIN_TILE_BYTES + p.digits * p.tokens * LIN_KB) +
                           (io_bends(a.io) ? ACT_TABLE_MAX : 0);
     const Launch l(dim3(p.ctas), THREADS, smem, s, overlap);
+    if (D == 4 && !w.gated && a.io.withhold) return cudaLaunchKernelEx(&l.cfg, linear_kernel<4, false, true>, a);
     return w.gated ? cudaLaunchKernelEx(&l.cfg, linear_kernel<D, true>, a)
                    : cudaLaunchKernelEx(&l.cfg, linear_kernel<D, false>, a);
 }
@@ -619,6 +627,7 @@ cudaError_t linear_configure() {
     if (e == cudaSuccess) e = configure_one<1, true>();
     if (e == cudaSuccess) e = configure_one<2, true>();
     if (e == cudaSuccess) e = configure_one<4, true>();
+    if (e == cudaSuccess) e = configure_one<4, false, true>();
     return e;
 }
 

@@ -34,15 +34,18 @@ struct TokenArgs {
     uint32_t slices;  // warps that share a unit's tokens: 1, 2 or 4
 };
 
-template <int D, bool GATED>
+// SELFTEST: with LinearIO::withhold (the instantiation of zkml_selftest_linear_wait alone).
+template <int D, bool GATED, bool SELFTEST = false>
 __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __grid_constant__ TokenArgs a) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * MAX_STAGES + 2];
-    __shared__ uint32_t tmem_base_s;
+    __shared__ uint32_t tmem_base_s, issued_s;
     __shared__ volatile uint32_t quit_s;
+    __shared__ volatile uint32_t missing_s;  // a block of the cluster gave up: its partial sums are not here
     constexpr int G = GROUP<D>;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t nt = blockIdx.x / a.parts, rank = blockIdx.x % a.parts;  // cluster dimension: parts
+    const int withhold = SELFTEST && nt == 0 && rank + 1 == a.parts ? a.io.withhold : 0;
     const uint32_t n_cols = D * a.tokens, stage_bytes = LIN_TILE_BYTES + n_cols * LIN_KB;
     const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
     const uint32_t full = smem_addr(bars), empty = full + 8 * MAX_STAGES, acc_full = empty + 8 * MAX_STAGES;
@@ -55,7 +58,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
     uint32_t cols = 32;
     while (cols < a.w.planes * n_cols) cols <<= 1;
     if (threadIdx.x == 0) {
-        quit_s = 0;
+        quit_s = missing_s = 0;
         for (uint32_t i = 0; i < a.stages; i++) {
             mbar_init(full + 8 * i, 1 + a.slices);  // the copy's issuer and the digit makers
             mbar_init(empty + 8 * i, 1);
@@ -89,7 +92,8 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             uint32_t st = 0, phase = 1, issued = 0;
             for (uint32_t u = 0; u < units; u++) {
                 if (u == a.stages) grid_dependency_wait();  // so that the waits' limit counts this grid's own time alone
-                if (!(ok = mbar_wait(empty + 8 * st, phase, &quit_s))) break;
+                if (!(ok = mbar_wait(empty + 8 * st, phase, &quit_s, a.io.wait_ns))) break;
+                if (SELFTEST && withhold == LIN_WITHHOLD_COPY && u + 1 == units) break;
                 uint32_t plane, kt;
                 tile_of(u, plane, kt);
                 mbar_expect_tx(full + 8 * st, LIN_TILE_BYTES);
@@ -99,14 +103,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
                 issued++;
                 if (++st == a.stages) st = 0, phase ^= 1;
             }
-            if (!ok) {  // copies in flight land before the block ends (their barriers also want the digits' arrival)
-                atomicOr(a.io.status, LIN_TIMEOUT);
-                volatile uint32_t never = 0;
-                for (uint32_t i = 0; i < min(issued, a.stages); i++) {
-                    const uint32_t u = issued - 1 - i;
-                    mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never);
-                }
-            }
+            issued_s = issued;
         }
     } else if (warp == 1) {
         if (lane == 0) {
@@ -114,7 +111,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             const uint32_t idesc = tc_idesc_s8(n_cols);
             uint32_t st = 0, phase = 0, kt_done = 0, plane = 0;
             for (uint32_t u = 0; u < units; u++) {
-                if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s))) break;
+                if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s, a.io.wait_ns))) break;
                 tc_fence_after();
                 const uint64_t da = tc_desc_k128(smem0 + st * stage_bytes);
                 const uint64_t db = tc_desc_k128(smem0 + st * stage_bytes + LIN_TILE_BYTES);
@@ -125,14 +122,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
                 if (++st == a.stages) st = 0, phase ^= 1;
                 if (++kt_done == k_len) kt_done = 0, plane++;
             }
-            if (ok) {
-                tc_commit(acc_full);
-            } else {
-                atomicOr(a.io.status, LIN_TIMEOUT);
-                volatile uint32_t never = 0;
-                tc_commit(drained);
-                mbar_wait(drained, 0, &never);
-            }
+            if (ok && !(SELFTEST && withhold == LIN_WITHHOLD_DONE)) tc_commit(acc_full);
         }
     } else {
         // ---- digit tiles: a lane takes 4 K of a token
@@ -171,7 +161,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             if (u_next < units) load(ahead, u_next);  // on its way while this one becomes digits
             const uint32_t st = u % a.stages, tile = smem0 + st * stage_bytes + LIN_TILE_BYTES;
             // the stage's last product is done
-            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ((u / a.stages) & 1) ^ 1, &quit_s));
+            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ((u / a.stages) & 1) ^ 1, &quit_s, a.io.wait_ns));
             if (!ok) break;
 #pragma unroll
             for (uint32_t i = 0; i < 2; i++) {
@@ -190,7 +180,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * st);
+            if (lane == 0 && !(SELFTEST && withhold == LIN_WITHHOLD_DIGITS && u + 1 == units)) mbar_arrive(full + 8 * st);
             u = u_next;
 #pragma unroll
             for (int i = 0; i < 2; i++) v[i] = ahead[i];
@@ -198,7 +188,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         if (bad) atomicOr(a.io.status, bad);
         // ---- this warp's quarter of the rows (warps 2 to 5): TMEM lanes 32 (warp % 4) and up
         if (maker < 4 && __all_sync(0xffffffffu, ok)) {
-            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, &quit_s));
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, &quit_s, a.io.wait_ns));
             tc_fence_after();
             if (ok) {
 #pragma unroll
@@ -230,6 +220,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
     const bool finisher = warp >= 2 && warp < 6;
     if (a.parts > 1) {
         const uint32_t holders = min(a.parts, 4u), held = (4 + holders - 1) / holders;
+        const uint32_t missing_at = smem_addr(const_cast<const uint32_t*>(&missing_s));
         cluster_wait();
         if (finisher && ok) {
             const uint32_t at = part_base + ((rank * held + quad / holders) * a.tokens * 32 + lane) * 4;
@@ -238,11 +229,13 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
 #pragma unroll
                 for (uint32_t t = 0; t < G; t++)
                     if (h * G + t < a.io.m) cluster_store(at + (h * G + t) * 128, quad % holders, z[h][t]);
+        } else if (finisher && lane == 0) {  // this warp gave up: the rows' holder must not finish without it
+            cluster_store(missing_at, quad % holders, 1);
         }
         __syncwarp();
         cluster_arrive();
         cluster_wait();
-        if (finisher && ok && quad % holders == rank) {
+        if (finisher && ok && quad % holders == rank && !missing_s) {
 #pragma unroll
             for (uint32_t h = 0; h < GROUPS; h++) {
                 if (h * G >= a.io.m) break;
@@ -273,6 +266,23 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (quit_s) {
+        // some role's wait ran out (all roles are done now): reported, and the copies and products still in
+        // flight end before the tensor memory and the block do
+        volatile uint32_t never = 0;
+        if (threadIdx.x == 0) {
+            atomicOr(a.io.status, LIN_TIMEOUT);
+            for (uint32_t i = 0; i < min(issued_s, a.stages); i++) {  // a barrier may lack the digits' arrival: then the limit ends it
+                const uint32_t u = issued_s - 1 - i;
+                mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never, a.io.wait_ns);
+            }
+        } else if (threadIdx.x == 32) {  // the products' issuer
+            tc_commit(drained);
+            mbar_wait(drained, 0, &never, a.io.wait_ns);
+        }
+        __syncwarp();
+        __syncthreads();
+    }
     if (warp == 2) tmem_free(tmem, cols);
 }
 
@@ -286,6 +296,7 @@ cudaError_t launch(const TokenArgs& a, const TokenPlan& p, cudaStream_t s, bool 
     attrs[1] = l.attr;
     l.cfg.attrs = attrs;
     l.cfg.numAttrs = overlap ? 2 : 1;
+    if (D == 4 && !a.w.gated && a.io.withhold) return cudaLaunchKernelEx(&l.cfg, linear_token_kernel<4, false, true>, a);
     return a.w.gated ? cudaLaunchKernelEx(&l.cfg, linear_token_kernel<D, true>, a)
                      : cudaLaunchKernelEx(&l.cfg, linear_token_kernel<D, false>, a);
 }
@@ -295,7 +306,8 @@ cudaError_t launch(const TokenArgs& a, const TokenPlan& p, cudaStream_t s, bool 
 cudaError_t linear_token_configure() {
     const void* kernels[] = {(const void*)linear_token_kernel<1, false>, (const void*)linear_token_kernel<2, false>,
                              (const void*)linear_token_kernel<4, false>, (const void*)linear_token_kernel<1, true>,
-                             (const void*)linear_token_kernel<2, true>,  (const void*)linear_token_kernel<4, true>};
+                             (const void*)linear_token_kernel<2, true>,  (const void*)linear_token_kernel<4, true>,
+                             (const void*)linear_token_kernel<4, false, true>};
     for (const void* k : kernels) {
         const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TOKEN_SMEM);
         if (e != cudaSuccess) return e;

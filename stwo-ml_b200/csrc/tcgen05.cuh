@@ -27,9 +27,9 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Waits for the phase `parity` of a barrier.  Gives up (false) when *quit is set, or after two
-// seconds, in which case it sets *quit so that the block's other waits end too.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* quit) {
+// Waits for the phase `parity` of a barrier.  Gives up (false) when *quit is set, or after limit_ns,
+// in which case it sets *quit so that the block's other waits end too.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* quit, uint64_t limit_ns) {
     if (mbar_try(bar, parity)) return true;
     uint64_t t0, t;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
@@ -38,7 +38,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         if (*quit) return false;
         if ((it & 63) == 0) {
             asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-            if (t - t0 > 2000000000ull) {
+            if (t - t0 > limit_ns) {
                 *quit = 1;
                 return false;
             }
