@@ -448,11 +448,15 @@ int zkml_linear_workspace(const zkml_linear *lin, size_t m, int x_bits, size_t *
 /* Launches the call and returns; the outputs follow in stream order.  It neither allocates nor
  * waits, so it can be captured into a CUDA graph.  An input word >= 2^31, or an activation
  * outside x_bits, marks the handle: the outputs of that call are then unspecified words, and
- * the next zkml_linear_check reports it. */
+ * a zkml_linear_check reports it. */
 int zkml_linear_forward(zkml_linear *lin, const zkml_linear_call *call);
-/* Waits for `stream` (NULL: the context's stream) and reports, once, whether a call since the
- * last check met such a value (ZKML_ERR_INVALID_ARG), or gave up on a wait inside its kernels and left
- * outputs unwritten (ZKML_ERR_TIMEOUT: two seconds without progress). */
+/* The same, then waits for the call's stream and reports what this call met, and nothing that other calls
+ * of the handle did: ZKML_ERR_INVALID_ARG for such a value, ZKML_ERR_TIMEOUT where a kernel gave up on a wait
+ * (two seconds without progress) and left outputs unwritten.  Refused while the stream is captured. */
+int zkml_linear_forward_checked(zkml_linear *lin, const zkml_linear_call *call);
+/* Waits for `stream` (NULL: the context's stream) and reports what calls of zkml_linear_forward met since the
+ * last check, with the same errors.  It covers the handle's calls on every stream: each finding is
+ * reported once, to whichever check comes first after it was made. */
 int zkml_linear_check(zkml_linear *lin, void *stream);
 
 /* ---- Stepwise product sumcheck (multi-GPU building block) -------------------

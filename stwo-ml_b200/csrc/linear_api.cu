@@ -1,6 +1,8 @@
 // C-ABI: forward operators with weights laid out once (zkml_linear_*).
 #include <algorithm>
 #include <atomic>
+#include <condition_variable>
+#include <mutex>
 #include <new>
 #include <string>
 
@@ -15,6 +17,13 @@ struct zkml_linear {
     const uint8_t* act_table[2] = {nullptr, nullptr};  // GELU, SiLU: on the device
     zk::DevBuf tiles;
     zk::DevBuf small;  // status words, column sums, per-row constants
+    // Status words: 0 collects what calls without a report of their own met; each call that reports by
+    // itself borrows one of the words from FIRST_SLOT on, all zero while nobody holds them.
+    static constexpr int FIRST_SLOT = 2, SLOTS = 62;
+    std::mutex slots_mutex;
+    std::condition_variable slot_free;
+    uint64_t slots_held = 0;
+    uint32_t* status(int word) const { return small.as<uint32_t>() + word; }
     void release() {
         tiles.release();
         small.release();
@@ -107,6 +116,51 @@ int status_error(uint32_t st) {
 }
 
 constexpr size_t STATUS_BYTES = 256;
+static_assert(4 * (zkml_linear::FIRST_SLOT + zkml_linear::SLOTS) <= STATUS_BYTES, "status words");
+
+// A status word of one call for its time; waits while all are in use.
+struct StatusSlot {
+    zkml_linear* lin;
+    int i = 0;
+    bool clean = true;  // zero again, or never written
+    explicit StatusSlot(zkml_linear* l) : lin(l) {
+        std::unique_lock<std::mutex> lock(l->slots_mutex);
+        const auto none = (uint64_t(1) << zkml_linear::SLOTS) - 1;
+        l->slot_free.wait(lock, [&] { return l->slots_held != none; });
+        while (l->slots_held >> i & 1) i++;
+        l->slots_held |= uint64_t(1) << i;
+    }
+    ~StatusSlot() {
+        if (!clean) return;  // a CUDA error left it unknown: it is not lent again
+        {
+            std::lock_guard<std::mutex> lock(lin->slots_mutex);
+            lin->slots_held &= ~(uint64_t(1) << i);
+        }
+        lin->slot_free.notify_one();
+    }
+    uint32_t* word() const { return lin->status(zkml_linear::FIRST_SLOT + i); }
+    // Waits for s and reports what was left in the word by then.
+    int report(cudaStream_t s) {
+        uint32_t st = 0;
+        clean = false;
+        ZK_CUDA(cudaMemcpyAsync(&st, word(), 4, cudaMemcpyDeviceToHost, s));
+        ZK_CUDA(cudaStreamSynchronize(s));
+        if (st) {
+            ZK_CUDA(cudaMemsetAsync(word(), 0, 4, s));
+            ZK_CUDA(cudaStreamSynchronize(s));
+        }
+        clean = true;
+        return status_error(st);
+    }
+};
+
+__global__ void take_status_kernel(uint32_t* status, uint32_t* out) { *out = atomicExch(status, 0u); }
+
+int refuse_capture(cudaStream_t s, const char* why) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    ZK_CUDA(cudaStreamIsCapturing(s, &cap));
+    return cap == cudaStreamCaptureStatusNone ? (int)ZKML_OK : set_error(ZKML_ERR_INVALID_ARG, why);
+}
 
 void set_shape(PackedWeights& w, size_t k, size_t n, bool gated) {
     w.k = (uint32_t)k;
@@ -173,10 +227,8 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     DeviceGuard guard(ctx->device);
     ZK_CUDA(guard.error);
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    ZK_CUDA(cudaStreamIsCapturing(s, &cap));
-    if (cap != cudaStreamCaptureStatusNone)
-        return set_error(ZKML_ERR_INVALID_ARG, "weights cannot be laid out while the stream is captured");
+    int rc = refuse_capture(s, "weights cannot be laid out while the stream is captured");
+    if (rc) return rc;
     zkml_linear* lin = new (std::nothrow) zkml_linear();
     if (!lin) return set_error(ZKML_ERR_OOM, "no host memory for the handle");
     struct Drop {
@@ -195,7 +247,6 @@ int create(zkml_ctx* ctx, const uint32_t* const* ws, const uint32_t* const* bias
     PackedWeights& w = lin->w;
     set_shape(w, k, n, parts == 2);
     const uint32_t* dev[4] = {};  // weights, then biases
-    int rc;
     for (int g = 0; g < 2 * parts; g++) {
         const bool is_bias = g >= parts;
         const uint32_t* src = is_bias ? biases[g - parts] : ws[g];
@@ -321,8 +372,9 @@ int zkml_linear_workspace(const zkml_linear* lin, size_t m, int x_bits, size_t* 
     return ZKML_OK;
 }
 
-// The call of zkml_linear_forward; withhold and wait_ns as in LinearIO.
-static int forward(zkml_linear* lin, const zkml_linear_call* c, int withhold, uint64_t wait_ns) {
+// The call of zkml_linear_forward with its status bits in `status`; withhold and wait_ns as in LinearIO.
+static int forward(zkml_linear* lin, const zkml_linear_call* c, uint32_t* status, int withhold = 0,
+                   uint64_t wait_ns = 0) {
     if (!lin || !c || !c->x || !c->out) return set_error(ZKML_ERR_INVALID_ARG, "NULL argument");
     size_t need = 0;
     int rc = zkml_linear_workspace(lin, c->m, c->x_bits, &need);
@@ -370,7 +422,7 @@ static int forward(zkml_linear* lin, const zkml_linear_call* c, int withhold, ui
     io.out = c->out;
     io.pre = c->pre;
     io.up = c->up;
-    io.status = lin->small.as<uint32_t>();
+    io.status = status;
     io.ldx = c->ldx;
     io.ld_res = c->ld_residual;
     io.ld_out = c->ld_out;
@@ -389,14 +441,31 @@ static int forward(zkml_linear* lin, const zkml_linear_call* c, int withhold, ui
     return ZKML_OK;
 }
 
-int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* call) { return forward(lin, call, 0, 0); }
+int zkml_linear_forward(zkml_linear* lin, const zkml_linear_call* call) {
+    return forward(lin, call, lin ? lin->status(0) : nullptr);
+}
+
+int zkml_linear_forward_checked(zkml_linear* lin, const zkml_linear_call* call) {
+    if (!lin || !call) return set_error(ZKML_ERR_INVALID_ARG, "NULL argument");
+    DeviceGuard guard(lin->ctx->device);
+    ZK_CUDA(guard.error);
+    cudaStream_t s = call->stream ? static_cast<cudaStream_t>(call->stream) : lin->ctx->stream;
+    int rc = refuse_capture(s, "a checked call waits for its stream, which is being captured");
+    if (rc) return rc;
+    StatusSlot slot(lin);
+    if ((rc = forward(lin, call, slot.word()))) {
+        slot.clean = rc == ZKML_ERR_INVALID_ARG;  // refused before any launch
+        return rc;
+    }
+    return slot.report(s);
+}
 
 int zkml_selftest_linear_wait(zkml_linear* lin, const zkml_linear_call* call, int withhold, uint32_t limit_ms) {
     if (!lin || !call) return set_error(ZKML_ERR_INVALID_ARG, "NULL argument");
     if (withhold < LIN_WITHHOLD_DONE || withhold > LIN_WITHHOLD_DIGITS || limit_ms == 0 || limit_ms > 1000 ||
         lin->w.gated || call->x_bits != 31)
         return set_error(ZKML_ERR_INVALID_ARG, "self-test: withhold 1 to 4, 1 to 1000 ms, plain weights, x_bits 31");
-    return forward(lin, call, withhold, limit_ms * 1000000ull);
+    return forward(lin, call, lin->status(0), withhold, limit_ms * 1000000ull);
 }
 
 int zkml_linear_check(zkml_linear* lin, void* stream) {
@@ -404,15 +473,14 @@ int zkml_linear_check(zkml_linear* lin, void* stream) {
     DeviceGuard guard(lin->ctx->device);
     ZK_CUDA(guard.error);
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : lin->ctx->stream;
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    ZK_CUDA(cudaStreamIsCapturing(s, &cap));
-    if (cap != cudaStreamCaptureStatusNone)
-        return set_error(ZKML_ERR_INVALID_ARG, "the check waits for the stream, which is being captured");
-    uint32_t st = 0;
-    ZK_CUDA(cudaMemcpyAsync(&st, lin->small.ptr, 4, cudaMemcpyDeviceToHost, s));
-    ZK_CUDA(cudaStreamSynchronize(s));
-    if (st) ZK_CUDA(cudaMemsetAsync(lin->small.ptr, 0, 4, s));
-    return status_error(st);
+    const int rc = refuse_capture(s, "the check waits for the stream, which is being captured");
+    if (rc) return rc;
+    StatusSlot slot(lin);
+    // read and cleared in one step: what calls on other streams set meanwhile is reported now or by the next check
+    take_status_kernel<<<1, 1, 0, s>>>(lin->status(0), slot.word());
+    ZK_CUDA(cudaGetLastError());
+    lin->ctx->launches++;
+    return slot.report(s);
 }
 
 }  // extern "C"

@@ -165,6 +165,7 @@ _SIGS = {
     "zkml_linear_workspace": (C.c_int, [C.c_void_p, C.c_size_t, C.c_int, C.POINTER(C.c_size_t)]),
     "zkml_linear_forward": (C.c_int, [C.c_void_p, C.c_void_p]),
     "zkml_selftest_linear_wait": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_uint32]),
+    "zkml_linear_forward_checked": (C.c_int, [C.c_void_p, C.c_void_p]),
     "zkml_linear_check": (C.c_int, [C.c_void_p, C.c_void_p]),
     "zkml_shm_exchange_open": (C.c_int, [C.c_char_p, C.c_int, C.c_int, C.c_size_t, C.c_uint64, C.c_void_p]),
     "zkml_shm_exchange_close": (C.c_int, [C.c_void_p]),

@@ -59,15 +59,17 @@ def _torch():
     return _torch_module
 
 
-_forward_fn = []
+_forward_fn = None
 
 
-def _forward():
-    """zkml_linear_forward with the handle as a plain integer and the packed call as bytes."""
-    if not _forward_fn:
-        addr = C.cast(lib().zkml_linear_forward, C.c_void_p).value
-        _forward_fn.append(C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_char_p)(addr))
-    return _forward_fn[0]
+def _forward(check):
+    """zkml_linear_forward (_checked) with the handle as a plain integer and the packed call as bytes."""
+    global _forward_fn
+    if _forward_fn is None:
+        sig = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_char_p)
+        _forward_fn = tuple(sig(C.cast(f, C.c_void_p).value)
+                            for f in (lib().zkml_linear_forward, lib().zkml_linear_forward_checked))
+    return _forward_fn[1 if check else 0]
 
 
 class _Weights:
@@ -172,8 +174,6 @@ class _Weights:
         if self._handle is None:
             raise InvalidArgument(1, "the weights were closed")
         torch = _torch()
-        if check and torch.cuda.is_current_stream_capturing():
-            raise InvalidArgument(1, "the check waits for the stream; pass check=False while it is captured")
         k, n = self.k, self.n
         xp, m, ldx = self._rows(x, k, "x")
         rp = ldr = op = ldo = pp = ldp = pu = ldu = ws = 0
@@ -216,16 +216,14 @@ class _Weights:
         stream = torch._C._cuda_getCurrentRawStream(self.device) or _STREAM_LEGACY
         call = _CALL.pack(xp, m, ldx, int(x_bits), _tag(activation), rp, ldr, op, ldo, pp, ldp, pu, ldu, ws, need, stream,
                           1)
-        rc = _forward()(self._handle.value, call)
+        rc = _forward(check)(self._handle.value, call)
         if rc:
             _check(rc)
-        if check:
-            self.check()
         return results
 
     def check(self) -> None:
-        """Waits for the current stream; raises if a call since the last check met a word >= 2^31 or an
-        activation that does not fit its x_bits."""
+        """Waits for the current stream; raises if a call with check=False, on any stream, met a word >= 2^31 or
+        an activation that does not fit its x_bits.  Each finding is raised once."""
         _check(lib().zkml_linear_check(self._handle, self._stream()))
 
     def _run(self, x, activation, residual, out, pre, up, keep, x_bits, check):
@@ -274,8 +272,8 @@ class LinearM31(_Weights):
         one row of n words for all; out / pre: int32 tensors to write, of any row stride (out may be the
         residual); x_bits: the width x is quantised to (8, 16, or 31 for any field element).
         check=True waits for the call and raises InvalidArgument for a word >= 2^31 or an x outside
-        x_bits; check=False returns at once (and can be captured into a CUDA graph), and check() reports
-        later."""
+        x_bits in this call; check=False returns at once (and can be captured into a CUDA graph), and
+        check() reports later."""
         return self._run(x, activation, residual, out, pre, None, keep, x_bits, check)
 
 

@@ -92,3 +92,118 @@ def test_refusals_of_the_wait_self_test():
                  (lin, x, out, "relu", 3), (lin, x, out, "none", 4), (lin, few, out[:1], "silu", 3), (gat, x, out, "none", 1)):
         assert selftest(*args) == 1, args[3:]
     lin.check()
+
+
+def test_a_call_answers_for_itself():
+    """What another call of the handle met is neither raised by a checked call nor lost with it."""
+    x, w = ints((4, 40), 31, 1), ints((40, 30), 8, 2)
+    bx = x.copy()
+    bx[3, 39] = 0x80000001
+    for m in (4, 1):  # the bad word is in the last row
+        lin, tx, bad, want = Z.LinearM31(dev(w)), dev(x[-m:]), dev(bx[-m:]), L.product(x[-m:], w)
+        s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s1):
+            lin(bad, check=False)
+        s1.synchronize()
+        with torch.cuda.stream(s2):
+            L.same(host(lin(tx)), want)  # checked, and right
+            with pytest.raises(Z.InvalidArgument, match="2\\^31"):
+                lin(bad)
+            with pytest.raises(Z.InvalidArgument, match="2\\^31"):
+                lin.check()  # the first call's, on s1
+            lin.check()
+            L.same(host(lin(tx)), want)
+
+
+def run_threads(n, work):
+    import threading
+    errors = []
+
+    def guarded(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                work(i)
+        except BaseException as e:  # noqa: B902 -- reported below
+            errors.append((i, repr(e)))
+
+    threads = [threading.Thread(target=guarded, args=(i,)) for i in range(n)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors[:3]
+
+
+@pytest.mark.parametrize("n_threads,calls", [(8, 100), (80, 10)])
+def test_checked_calls_of_many_threads(n_threads, calls):
+    """Exactly the calls with a bad word raise, also with more callers than the handle has status words."""
+    x, w = ints((9, 200), 8, 1), ints((200, 130), 8, 2)
+    lin, tx, want = Z.LinearM31(dev(w)), dev(x), L.product(x, w)
+    bad = tx.clone()
+    bad[:, 7] = 1 << 20  # beyond 8 bits
+    torch.cuda.synchronize()
+
+    def work(i):
+        for j in range(calls):
+            m = 1 + (i + j) % 9
+            if (i + j) % 2:
+                with pytest.raises(Z.InvalidArgument, match="x_bits"):
+                    lin(bad[:m], x_bits=8)
+            else:
+                L.same(host(lin(tx[:m], x_bits=8)), want[:m])
+
+    run_threads(n_threads, work)
+    lin.check()
+
+
+def test_checks_of_several_threads_lose_nothing():
+    """Every finding is raised by one of the checks that run at the same time."""
+    w = ints((40, 30), 8, 2)
+    lin = Z.LinearM31(dev(w))
+    bad = torch.full((1, 40), -1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    raised, done = [0, 0, 0], []
+
+    def check(i):
+        try:
+            lin.check()
+        except Z.InvalidArgument:
+            raised[i] += 1
+
+    def work(i):
+        import time
+        if i:
+            while not done:
+                check(i)
+            return
+        try:
+            for _ in range(300):
+                before = sum(raised)
+                lin(bad, check=False)
+                torch.cuda.current_stream().synchronize()
+                check(0)
+                end = time.monotonic() + 5
+                while sum(raised) == before:
+                    assert time.monotonic() < end, "a finding was lost"
+                    time.sleep(0)
+        finally:
+            done.append(1)
+
+    run_threads(3, work)
+
+
+def test_a_checked_call_is_refused_in_a_capture():
+    """Before anything of it is launched, and the capture goes on."""
+    x, w = ints((9, 200), 31, 1), ints((200, 130), 8, 2)
+    lin, tx = Z.LinearM31(dev(w)), dev(x)
+    lin(tx)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(Z.InvalidArgument, match="captured"):
+            lin(tx)
+        with pytest.raises(Z.InvalidArgument, match="captured"):
+            lin.check()
+        y = lin(tx, check=False)
+    g.replay()
+    torch.cuda.synchronize()
+    L.same(host(y), L.product(x, w))
+    lin.check()
