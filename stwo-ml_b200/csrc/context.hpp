@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -133,7 +134,7 @@ struct zkml_ctx {
     // Queued look-ahead kernels that wait for a challenge launch as programmatic
     // dependents of the kernel before them (ZKML_LA_PDL=0: plain launches).
     bool la_pdl = true;
-    uint64_t launches = 0;
+    std::atomic<uint64_t> launches{0};  // forward operators count here from several threads at once
     // scratch
     zk::DevBuf a_in, b_in;          // device copies of host inputs
     zk::DevBuf fa, fb;              // QM31 sumcheck vectors
@@ -155,7 +156,7 @@ struct zkml_ctx {
     size_t pack_host_bytes = 0;
     zk::DevBuf pack_dev;            // packed bytes on the device
     cudaEvent_t pack_event = nullptr;  // after the last upload's copies
-    uint64_t h2d_bytes = 0;         // host -> device bytes of the matrix uploads
+    std::atomic<uint64_t> h2d_bytes{0};  // host -> device bytes of the matrix uploads (as launches)
     // stepwise product-sumcheck session (zkml_sumcheck_*)
     zk::DevBuf sc_a, sc_b;          // staged M31 inputs
     const uint32_t* sc_a32 = nullptr;

@@ -872,8 +872,8 @@ int zkml_ctx_destroy(zkml_ctx* ctx) {
 }
 
 int zkml_ctx_device(const zkml_ctx* ctx) { return ctx ? ctx->device : -1; }
-uint64_t zkml_ctx_kernel_launches(const zkml_ctx* ctx) { return ctx ? ctx->launches : 0; }
-uint64_t zkml_ctx_h2d_bytes(const zkml_ctx* ctx) { return ctx ? ctx->h2d_bytes : 0; }
+uint64_t zkml_ctx_kernel_launches(const zkml_ctx* ctx) { return ctx ? ctx->launches.load() : 0; }
+uint64_t zkml_ctx_h2d_bytes(const zkml_ctx* ctx) { return ctx ? ctx->h2d_bytes.load() : 0; }
 
 int zkml_ctx_enable_timing(zkml_ctx* ctx, int enable) {
     if (!ctx) return set_error(ZKML_ERR_INVALID_ARG, "ctx is NULL");

@@ -207,3 +207,46 @@ def test_a_checked_call_is_refused_in_a_capture():
     torch.cuda.synchronize()
     L.same(host(y), L.product(x, w))
     lin.check()
+
+
+HAMMER = """
+#include <atomic>
+#include <thread>
+#include <vector>
+extern "C" int hammer(int (*forward)(void*, const void*), void* lin, void* const* calls, int threads, int times) {
+    std::atomic<int> failed{0}, ready{0};
+    std::vector<std::thread> all;
+    for (int t = 0; t < threads; t++)
+        all.emplace_back([&, t] {
+            ready++;
+            while (ready < threads) {}
+            for (int i = 0; i < times; i++) failed += forward(lin, calls[t]) != 0;
+        });
+    for (std::thread& t : all) t.join();
+    return failed;
+}
+"""
+
+
+def test_launches_of_several_threads_are_all_counted(tmp_path):
+    """Native threads, which no interpreter lock keeps apart."""
+    import subprocess
+    (tmp_path / "hammer.cpp").write_text(HAMMER)
+    subprocess.run(["g++", "-O2", "-shared", "-fPIC", "-pthread", "-o", str(tmp_path / "hammer.so"),
+                    str(tmp_path / "hammer.cpp")], check=True)
+    w = ints((40, 30), 8, 2)
+    lin, tx, threads, times = Z.LinearM31(dev(w)), dev(ints((1, 40), 31, 1)), 8, 5000
+    out = torch.empty(threads, 30, dtype=torch.int32, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(threads)]
+    calls = [LinearCall(x=tx.data_ptr(), m=1, ldx=40, x_bits=31, out=out[t].data_ptr(), ld_out=30,
+                        stream=streams[t].cuda_stream, pointers_checked=1) for t in range(threads)]
+    torch.cuda.synchronize()
+    before = Z.context(0).kernel_launches()
+    failed = C.CDLL(str(tmp_path / "hammer.so")).hammer(
+        C.cast(Z.lib().zkml_linear_forward, C.c_void_p), lin._handle,
+        (C.c_void_p * threads)(*(C.addressof(c) for c in calls)), threads, times)
+    torch.cuda.synchronize()
+    assert failed == 0
+    assert Z.context(0).kernel_launches() - before == threads * times  # one launch a call for a single token
+    assert torch.equal(out, lin(tx).expand(threads, 30))
+    lin.check()
