@@ -82,19 +82,18 @@ class _Weights:
         self.device = int(device)
         self._handle = None
         self._need = {}
-        keep, ptrs, strides = [], [], []
+        keep, ptrs = [], []
         for w in weights:
             if len(w.shape) != 2:
                 raise InvalidArgument(1, "a weight is a matrix")
             if tuple(w.shape) != tuple(first.shape):
                 raise InvalidArgument(1, "the weights of a gated block have the same shape")
-        if any(_strides(w) != _strides(first) for w in weights):
+        weights = [self._words(w, "weight") for w in weights]
+        if any(_strides(w) != _strides(weights[0]) for w in weights):
             weights = [w.contiguous() if _is_tensor(w) else np.ascontiguousarray(w) for w in weights]
         for w in weights:
-            w = self._words(w, "weight")
             keep.append(w)
             ptrs.append(_pointer(w))
-            strides.append(_strides(w))
         self.k, self.n = int(first.shape[0]), int(first.shape[1])
         for b in biases:
             if b is None:
@@ -108,7 +107,7 @@ class _Weights:
         self._ctx = context(self.device)
         h = C.c_void_p()
         create = lib().zkml_linear_create_gated if len(weights) == 2 else lib().zkml_linear_create
-        rs, cs = strides[0]
+        rs, cs = _strides(weights[0])
         _check(create(self._ctx.handle, *ptrs[:len(weights)], self.k, self.n, rs, cs, *ptrs[len(weights):],
                       self._stream(), C.byref(h)))
         self._handle = h
@@ -136,7 +135,9 @@ class _Weights:
             x = np.asarray(x)
             if x.dtype not in (np.uint32, np.int32):
                 raise InvalidArgument(1, f"{name}: M31 words are uint32 or int32")
-            return x if all(s >= 0 for s in x.strides) else np.ascontiguousarray(x)
+            # the library takes addresses and strides in whole words, upwards
+            whole = x.ctypes.data % x.itemsize == 0 and all(s >= 0 and s % x.itemsize == 0 for s in x.strides)
+            return x if whole else np.array(x, order="C")
         torch = _torch()
         if x.dtype not in (torch.int32, torch.uint32):
             raise InvalidArgument(1, f"{name}: M31 words are int32 or uint32")

@@ -8,6 +8,7 @@ import torch
 
 import linear_plain as L
 import zkml_b200 as Z
+from test_linear_checks import awkward_words
 from test_linear_gpu import LinearCall, TAGS, dev, host, ints
 
 pytestmark = pytest.mark.gpu
@@ -250,3 +251,16 @@ def test_launches_of_several_threads_are_all_counted(tmp_path):
     assert Z.context(0).kernel_launches() - before == threads * times  # one launch a call for a single token
     assert torch.equal(out, lin(tx).expand(threads, 30))
     lin.check()
+
+
+def test_host_weights_of_any_byte_stride():
+    """Fields of records, odd addresses, both alone and beside a plain matrix in a gated block."""
+    x, w, up, b = ints((3, 90), 31, 1), ints((90, 50), 8, 2), ints((90, 50), 8, 3), ints((50,), 31, 4)
+    want = L.linear(x, w, b)[0]
+    h, _, _, unsure = L.gated(x, w, up)
+    wide = np.zeros((90, 100), np.uint32)[:, ::2]  # as many whole words from one to the next as a record's field
+    wide[...] = up
+    for weight, bias in zip(awkward_words(w), awkward_words(np.repeat(b[None], 2, 0))):
+        L.same(host(Z.LinearM31(weight, bias[1])(dev(x))), want)
+        for other in (up, wide, dev(up), np.asfortranarray(up)):
+            L.same(host(Z.GatedLinearM31(weight, other)(dev(x))), h, unsure)
