@@ -99,7 +99,7 @@ bool linear_token_plan(const PackedWeights& w, uint32_t m, int x_bits, int num_s
 cudaError_t launch_linear_token(const PackedWeights& w, const TokenPlan& p, const LinearIO& io, cudaStream_t s,
                                 bool overlap);
 cudaError_t linear_token_configure();
-cudaError_t linear_configure();  // per device, before the first launch
+cudaError_t linear_configure(cudaStream_t s);  // per device, before the first launch; uploads tables on s
 // The current device's copy of the segment table, NULL for other activations.
 cudaError_t linear_act_table(int tag, const uint8_t** out);
 // overlap: the weights were in place before the work now queued on s, so they may be read while

@@ -170,6 +170,20 @@ void set_shape(PackedWeights& w, size_t k, size_t n, bool gated) {
     w.n_tiles = (uint32_t)((n + lin_outputs_per_tile(gated) - 1) / lin_outputs_per_tile(gated));
 }
 
+// What the kernels need once per device, in place when this returns: readers of the tables run on any stream.
+int configure(int device, cudaStream_t s) {
+    static std::mutex one;
+    static std::atomic<bool> done[64];
+    if (device < 64 && done[device].load(std::memory_order_acquire)) return ZKML_OK;
+    std::lock_guard<std::mutex> lock(one);
+    if (device < 64 && done[device].load(std::memory_order_acquire)) return ZKML_OK;
+    ZK_CUDA(linear_configure(s));
+    ZK_CUDA(linear_token_configure());
+    ZK_CUDA(cudaStreamSynchronize(s));
+    if (device < 64) done[device].store(true, std::memory_order_release);
+    return ZKML_OK;
+}
+
 // Lays out weights of shape w from device memory (src: the weights, then the biases) and waits;
 // *bad: a word >= 2^31 was among them.  Signed bytes in most models: one plane is packed, and again
 // with more where a value needs them.
@@ -177,12 +191,7 @@ int lay_out(zkml_ctx* ctx, PackedWeights& w, const uint32_t* const src[4], size_
             DevBuf& small, cudaStream_t s, uint32_t* bad) {
     const size_t slots = (size_t)w.n_tiles * LIN_ROWS, plane = (size_t)w.n_tiles * w.k_tiles * LIN_TILE_BYTES;
     int rc;
-    static std::atomic<bool> configured[64];
-    if (ctx->device >= 64 || !configured[ctx->device].load(std::memory_order_relaxed)) {
-        ZK_CUDA(linear_configure());
-        ZK_CUDA(linear_token_configure());
-        if (ctx->device < 64) configured[ctx->device].store(true, std::memory_order_relaxed);
-    }
+    if ((rc = configure(ctx->device, s))) return rc;
     if ((rc = small.ensure(STATUS_BYTES + slots * 16))) return rc;
     uint32_t* const status = small.as<uint32_t>();
     unsigned long long* const sums = reinterpret_cast<unsigned long long*>(small.as<uint8_t>() + STATUS_BYTES);

@@ -617,10 +617,12 @@ cudaError_t linear_act_table(int tag, const uint8_t** out) {
     return e;
 }
 
-cudaError_t linear_configure() {
-    cudaError_t e = cudaMemcpyToSymbol(act_tables, act_segment_table(2), act_table_bytes(2), 0);
+cudaError_t linear_configure(cudaStream_t s) {
+    cudaError_t e = cudaMemcpyToSymbolAsync(act_tables, act_segment_table(2), act_table_bytes(2), 0,
+                                            cudaMemcpyHostToDevice, s);
     if (e == cudaSuccess)
-        e = cudaMemcpyToSymbol(act_tables, act_segment_table(5), act_table_bytes(5), act_table_bytes(2));
+        e = cudaMemcpyToSymbolAsync(act_tables, act_segment_table(5), act_table_bytes(5), act_table_bytes(2),
+                                    cudaMemcpyHostToDevice, s);
     if (e == cudaSuccess) e = configure_one<1, false>();
     if (e == cudaSuccess) e = configure_one<2, false>();
     if (e == cudaSuccess) e = configure_one<4, false>();

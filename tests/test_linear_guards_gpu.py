@@ -264,3 +264,46 @@ def test_host_weights_of_any_byte_stride():
         L.same(host(Z.LinearM31(weight, bias[1])(dev(x))), want)
         for other in (up, wide, dev(up), np.asfortranarray(up)):
             L.same(host(Z.GatedLinearM31(weight, other)(dev(x))), h, unsure)
+
+
+FIRST_HANDLE = """
+import ctypes as C
+import sys
+sys.path[:0] = {path!r}
+import numpy as np
+import torch
+import linear_plain as L
+import zkml_b200 as Z
+from test_linear_gpu import dev, host, ints
+
+Z.context(0)
+x, w = ints((9, 300), 8, 1), ints((300, 130), 8, 2)
+tx, side, handle = dev(x), torch.cuda.Stream(), C.c_uint64()
+assert int(torch.cuda.cudart().cudaStreamCreate(C.addressof(handle))) == 0  # a stream that orders with the legacy one
+blocking, g = torch.cuda.ExternalStream(handle.value), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g, stream=blocking, capture_error_mode="relaxed"):
+    twice = tx + tx
+    with torch.cuda.stream(side):
+        lin = Z.LinearM31(w)
+with torch.cuda.stream(side):
+    for m in (9, 1):  # both kernels read the tables
+        y, _, unsure = L.linear(x[:m], w, None, 5)
+        L.same(host(lin(tx[:m], activation="silu", x_bits=8)), y, unsure)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(twice, tx + tx)
+print("ok")
+"""
+
+
+def test_the_first_handle_uses_its_own_stream_alone():
+    """A process's first handle uploads the activation tables; made beside the capture of a stream that orders
+    with the legacy stream, it neither fails nor ends the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parents[1]
+    path = [str(root), str(root / "tests"), str(root / "stwo-ml_b200")]
+    r = subprocess.run([sys.executable, "-c", FIRST_HANDLE.format(path=path)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout[-2000:] + r.stderr[-4000:]
