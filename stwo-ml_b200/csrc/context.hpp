@@ -108,11 +108,13 @@ struct OpeningScratch {
         for (DevBuf* b : all) b->release();
     }
 };
-// Device scratch of the forward pass's products with weights used once (grown on demand).
+// Device scratch of the forward pass's products with weights used once (grown on demand, given back after a
+// pass where it is large).
 struct LinearScratch {
     DevBuf tiles, small;  // as a zkml_linear's
     DevBuf met;           // what the calls of a run met (status bits)
     DevBuf workspace;
+    size_t bytes() const { return tiles.bytes + small.bytes + met.bytes + workspace.bytes; }
     void release() {
         DevBuf* all[] = {&tiles, &small, &met, &workspace};
         for (DevBuf* b : all) b->release();

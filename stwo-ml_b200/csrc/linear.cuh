@@ -110,7 +110,7 @@ cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const Lin
 // One product with weights that are used once (the chain prover's forward pass): lays w (k x n,
 // row major, host or device memory) out in the context's scratch and runs the call on its stream.
 // x, residual, pre and out are dense device matrices; pre may be NULL.  ZKML_ERR_OOM leaves
-// nothing done.  A run of calls is opened by _begin and closed by _end, which waits for the stream
+// nothing done and no scratch of its own held.  A run of calls is opened by _begin and closed by _end, which waits for the stream
 // and reports what the calls met.
 int linear_once_begin(::zkml_ctx* ctx);
 int linear_once_end(::zkml_ctx* ctx);

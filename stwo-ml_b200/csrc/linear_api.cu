@@ -299,14 +299,33 @@ int linear_once_begin(zkml_ctx* ctx) {
     return ZKML_OK;
 }
 
+// Scratch of at most this many bytes stays with the context between forward passes; more is given back, so that
+// what follows (reductions, commitments) has the memory that it had before.
+constexpr size_t ONCE_KEEP = (size_t)64 << 20;
+
 int linear_once_end(zkml_ctx* ctx) {
     uint32_t st = 0;
     ZK_CUDA(cudaMemcpyAsync(&st, ctx->lin.met.ptr, 4, cudaMemcpyDeviceToHost, ctx->stream));
     ZK_CUDA(cudaStreamSynchronize(ctx->stream));
+    if (ctx->lin.bytes() > ONCE_KEEP) ctx->lin.release();
     return status_error(st);
 }
 
+static int once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint32_t* w, size_t n, int activation,
+                const uint32_t* residual, uint32_t* pre, uint32_t* out);
+
 int linear_once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint32_t* w, size_t n, int activation,
+                const uint32_t* residual, uint32_t* pre, uint32_t* out) {
+    const int rc = once(ctx, x, m, k, w, n, activation, residual, pre, out);
+    if (rc) {  // the caller may need the memory for another way (cudaFree waits for queued work); met stays
+        ctx->lin.tiles.release();
+        ctx->lin.small.release();
+        ctx->lin.workspace.release();
+    }
+    return rc;
+}
+
+static int once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint32_t* w, size_t n, int activation,
                 const uint32_t* residual, uint32_t* pre, uint32_t* out) {
     if (m > (1u << 30) || k > (1u << 30) || n > (1u << 30) || m * k > ((size_t)1 << 34) || k * n > ((size_t)1 << 34))
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");

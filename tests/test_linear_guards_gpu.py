@@ -307,3 +307,22 @@ def test_the_first_handle_uses_its_own_stream_alone():
     path = [str(root), str(root / "tests"), str(root / "stwo-ml_b200")]
     r = subprocess.run([sys.executable, "-c", FIRST_HANDLE.format(path=path)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout[-2000:] + r.stderr[-4000:]
+
+
+def test_a_forward_pass_gives_large_scratch_back():
+    """Weights of any field element (four bytes each when laid out, 64 MiB and more) leave no more of the
+    memory taken than signed bytes of the same shape do."""
+    d = 4096
+    x = L.words(np.random.default_rng(1).integers(-50, 50, (2, d)))
+
+    def free_after(w):
+        p = Z.prove_gkr_chain(x, [("linear", w)], n_queries=2)
+        torch.cuda.synchronize()
+        return torch.cuda.mem_get_info()[0], p.io_commitment
+
+    narrow, wide = ints((d, d), 8, 1), ints((d, d), 31, 2)
+    free_after(narrow)
+    before, io = free_after(narrow)
+    after, wide_io = free_after(wide)
+    assert after >= before
+    assert free_after(narrow)[1] == io and free_after(wide)[1] == wide_io
