@@ -108,15 +108,13 @@ struct OpeningScratch {
         for (DevBuf* b : all) b->release();
     }
 };
-// Device scratch of the forward pass's products with weights used once (grown on demand, given back after a
-// pass where it is large).
+// Device scratch of the forward pass's products with weights used once (grown on demand).
 struct LinearScratch {
-    DevBuf tiles, small;  // as a zkml_linear's
-    DevBuf met;           // what the calls of a run met (status bits)
+    DevBuf small;  // as a zkml_linear's
+    DevBuf met;    // what the calls of a run met (status bits)
     DevBuf workspace;
-    size_t bytes() const { return tiles.bytes + small.bytes + met.bytes + workspace.bytes; }
     void release() {
-        DevBuf* all[] = {&tiles, &small, &met, &workspace};
+        DevBuf* all[] = {&small, &met, &workspace};
         for (DevBuf* b : all) b->release();
     }
 };

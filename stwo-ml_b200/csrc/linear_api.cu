@@ -299,15 +299,10 @@ int linear_once_begin(zkml_ctx* ctx) {
     return ZKML_OK;
 }
 
-// Scratch of at most this many bytes stays with the context between forward passes; more is given back, so that
-// what follows (reductions, commitments) has the memory that it had before.
-constexpr size_t ONCE_KEEP = (size_t)64 << 20;
-
 int linear_once_end(zkml_ctx* ctx) {
     uint32_t st = 0;
     ZK_CUDA(cudaMemcpyAsync(&st, ctx->lin.met.ptr, 4, cudaMemcpyDeviceToHost, ctx->stream));
     ZK_CUDA(cudaStreamSynchronize(ctx->stream));
-    if (ctx->lin.bytes() > ONCE_KEEP) ctx->lin.release();
     return status_error(st);
 }
 
@@ -318,7 +313,7 @@ int linear_once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint
                 const uint32_t* residual, uint32_t* pre, uint32_t* out) {
     const int rc = once(ctx, x, m, k, w, n, activation, residual, pre, out);
     if (rc) {  // the caller may need the memory for another way (cudaFree waits for queued work); met stays
-        ctx->lin.tiles.release();
+        ctx->op.bmle.release();
         ctx->lin.small.release();
         ctx->lin.workspace.release();
     }
@@ -331,6 +326,9 @@ static int once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint
         return set_error(ZKML_ERR_INVALID_ARG, "matrix too large");
     if (m * n > ((size_t)1 << 34)) return set_error(ZKML_ERR_OOM, "output too large to be tiled");
     LinearScratch& b = ctx->lin;
+    // Weights are laid out where the proof later writes the same weight's evaluations (16 bytes an entry) to
+    // open it: no memory of their own is held beside what the proof needs anyway.
+    DevBuf& tiles = ctx->op.bmle;
     cudaStream_t s = ctx->stream;
     const void* dev = nullptr;
     PackedWeights p;
@@ -338,7 +336,7 @@ static int once(zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint
     uint32_t bad = 0;
     int rc = device_view(ctx, w, k * n * 4, ctx->b_in, &dev);
     const uint32_t* src[4] = {static_cast<const uint32_t*>(dev), nullptr, nullptr, nullptr};
-    if (!rc) rc = lay_out(ctx, p, src, n, 1, b.tiles, b.small, s, &bad);
+    if (!rc) rc = lay_out(ctx, p, src, n, 1, tiles, b.small, s, &bad);
     if (rc) return rc;
     if (bad) return set_error(ZKML_ERR_INVALID_ARG, "matmul_m31: input value >= 2^31 is not an M31 element");
     const Choice& c = choose(p, (uint32_t)m, 31, ctx->num_sms);
