@@ -147,11 +147,13 @@ class _Weights:
 
     def _rows(self, x, width, name, m=None):
         """(pointer, rows, row stride) of a matrix of words on this device; one row may be 1-D."""
-        if x.is_cuda and x.dtype is _torch().int32 and x.get_device() == self.device and x.dim() == 2:
+        if getattr(x, "is_cuda", False) and x.dtype is _torch().int32 and x.get_device() == self.device and x.dim() == 2:
             rows, cols = x.shape
             ld, one = x.stride()
             if cols == width and (one == 1 or width == 1) and rows and (m is None or rows == m):
                 return x.data_ptr(), rows, ld if rows > 1 else width  # the common form, in a few attribute reads
+        if not _is_tensor(x):
+            raise InvalidArgument(1, f"{name}: arguments beside a tensor x are tensors on cuda:{self.device} too")
         x = self._words(x, name)
         if not x.dim() or x.shape[-1] != width:
             raise InvalidArgument(1, f"{name} has rows of {width} words")
@@ -179,7 +181,7 @@ class _Weights:
         xp, m, ldx = self._rows(x, k, "x")
         rp = ldr = op = ldo = pp = ldp = pu = ldu = ws = 0
         if residual is not None:
-            if residual.dim() == 1 and m != 1:
+            if _is_tensor(residual) and residual.dim() == 1 and m != 1:
                 residual = residual.unsqueeze(0).expand(m, n)  # one row for every token
             rp, _, ldr = self._rows(residual, n, "residual", m)
         if out is None or (keep and (pre is None or (up is None and self._gated))):

@@ -44,3 +44,10 @@ def test_words_of_arrays_in_whole_words():
         np.testing.assert_array_equal(got.astype(np.uint32), w)
     for v in (w, w.T, w[::2, 1:], np.broadcast_to(w[0], (5, 7))):  # read in place
         assert _bare()._words(v, "weight") is v
+
+
+def test_an_array_beside_a_tensor_is_refused():
+    w = _bare()
+    for rows in (np.zeros((3, 6), np.uint32), np.zeros(6, np.int32), [[0] * 6]):
+        with pytest.raises(Z.InvalidArgument, match="tensors on cuda:0"):
+            w._rows(rows, 6, "residual")

@@ -326,3 +326,14 @@ def test_a_forward_pass_gives_large_scratch_back():
     after, wide_io = free_after(wide)
     assert after >= before
     assert free_after(narrow)[1] == io and free_after(wide)[1] == wide_io
+
+
+def test_arrays_and_tensors_in_one_call():
+    x, w, r = ints((4, 40), 31, 1), ints((40, 30), 8, 2), ints((4, 30), 31, 3)
+    lin, tx = Z.LinearM31(dev(w)), dev(x)
+    for args in (dict(residual=r), dict(residual=r[0]), dict(out=np.zeros((4, 30), np.uint32)), dict(pre=r)):
+        with pytest.raises(Z.InvalidArgument):
+            lin(tx, **args)
+    with pytest.raises(Z.InvalidArgument):
+        lin(x, out=torch.zeros(4, 30, dtype=torch.int32, device="cuda"))
+    L.same(lin(x, residual=dev(r)), L.linear(x, w, None, 0, r)[0])
