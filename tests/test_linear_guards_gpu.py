@@ -337,3 +337,87 @@ def test_arrays_and_tensors_in_one_call():
     with pytest.raises(Z.InvalidArgument):
         lin(x, out=torch.zeros(4, 30, dtype=torch.int32, device="cuda"))
     L.same(lin(x, residual=dev(r)), L.linear(x, w, None, 0, r)[0])
+
+
+SEGMENT = 1023 * 128  # K of one 32-bit accumulation
+
+
+def extreme_rows(m, k, x_bits, rng):
+    """Rows of two constants each (at the ends of the digits' range in most), and where the second begins."""
+    ends = {8: [-128, 127], 16: [-32768, 32767, -32640, 128 - 128 * 257],
+            31: [-(1 << 30) + 1, (1 << 30) - 1, 128 - 128 * 65793, 128 + 127 * 65793]}[x_bits]
+    first = np.array([ends[i % len(ends)] for i in range(m)], np.int64)
+    second = np.array([ends[(i // len(ends)) % len(ends)] for i in range(m)], np.int64)
+    at = rng.integers(0, k, m)
+    at[0] = k
+    x = torch.empty(m, k, dtype=torch.int32, device="cuda")
+    for i in range(m):
+        x[i, :at[i]], x[i, at[i]:] = int(L.words(first[i])), int(L.words(second[i]))
+    return x, first, second, at
+
+
+def sliding_weights(k, n, top, rng):
+    """w[t][j] = v[t + j], v at one end of the signed bytes but for a few: its column sums come from prefix sums."""
+    v = np.full(k + n - 1, top, np.int64)
+    v[rng.integers(0, v.size, 64)] = rng.integers(-128, 128, 64)
+    d = dev(L.words(v))
+    return torch.as_strided(d, (k, n), (1, 1)), np.concatenate([[0], np.cumsum(v)])
+
+
+def sliding_product(rows, sums, k, n):
+    _, first, second, at = rows
+    j = np.arange(n)
+    head = sums[at[:, None] + j] - sums[j]             # sum of w[t][j] over t < at
+    tail = sums[k + j] - sums[at[:, None] + j]
+    assert np.abs(sums).max() < 1 << 32                # times a first or second below 2^31: 63 bits
+    return (first[:, None] * head % P + second[:, None] * tail % P) % P
+
+
+@pytest.mark.parametrize("top", [-128, 127])
+@pytest.mark.parametrize("m,x_bits,extra", [(16, 31, 0), (16, 31, 2), (16, 8, 0), (16, 8, 2), (16, 16, 2), (40, 31, 2), (1, 31, 0)])
+def test_accumulations_are_cut_where_32_bits_end(m, x_bits, extra, top):
+    """Whole tiles of K past one accumulation, and (extra tiles) shares of cut tiles as long as that."""
+    k, n = 1100 * 128, 128 * (torch.cuda.get_device_properties(0).multi_processor_count + extra)
+    assert k > SEGMENT and 128 * 128 * (k - 64) > 1 << 31  # digits and weights of -128: past 32 bits without a cut
+    rng = np.random.default_rng(500 + m + x_bits + extra + top)
+    rows, (w, sums) = extreme_rows(m, k, x_bits, rng), sliding_weights(k, n, top, rng)
+    L.same(host(Z.LinearM31(w)(rows[0], x_bits=x_bits)), sliding_product(rows, sums, k, n))
+
+
+@pytest.mark.parametrize("extra", [0, 2])
+def test_gated_accumulations_are_cut_where_32_bits_end(extra):
+    m, k, n = 16, 1100 * 128, 64 * (torch.cuda.get_device_properties(0).multi_processor_count + extra)
+    rng = np.random.default_rng(extra)
+    rows, (wg, sg), (wu, su) = extreme_rows(m, k, 31, rng), sliding_weights(k, n, -128, rng), sliding_weights(k, n, 127, rng)
+    g, u = sliding_product(rows, sg, k, n), sliding_product(rows, su, k, n)
+    got = Z.GatedLinearM31(wg, wu)(rows[0], activation="relu", keep=True)
+    for a, want in zip(got, (L.activation(g, 1)[0] * u % P, g, u)):
+        L.same(host(a), want)
+
+
+@pytest.mark.parametrize("m,x_bits", [(1, 31), (8, 31), (3, 8), (8, 16)])
+@pytest.mark.parametrize("top", [-128, 127])
+def test_shares_of_a_cluster_up_to_one_accumulation(m, x_bits, top):
+    """A few tokens, K over six blocks: each share is the longest that the kernel for few tokens takes."""
+    k, n = 6137 * 128, 100
+    assert SEGMENT - 256 < k // 6 <= SEGMENT
+    rng = np.random.default_rng(500 + m + x_bits + top)
+    rows, (w, sums) = extreme_rows(m, k, x_bits, rng), sliding_weights(k, n, top, rng)
+    L.same(host(Z.LinearM31(w)(rows[0], x_bits=x_bits)), sliding_product(rows, sums, k, n))
+
+
+@pytest.mark.parametrize("m,x_bits", [(1, 31), (4, 31), (8, 31), (2, 16), (8, 8)])
+@pytest.mark.parametrize("w_bits", [16, 24, 31])
+@pytest.mark.parametrize("k", [1024, 2600])
+def test_wide_weights_over_a_cluster(k, w_bits, m, x_bits):
+    """Several planes of weights where K is shared by the blocks of a cluster."""
+    n = 200
+    x, w, w2, r = ints((m, k), x_bits, 1), ints((k, n), w_bits, 2), ints((k, n), w_bits, 3), ints((m, n), 31, 4)
+    y, z, unsure = L.linear(x, w, None, 5, r)
+    got = Z.LinearM31(dev(w))(dev(x), activation="silu", residual=dev(r), keep=True, x_bits=x_bits)
+    L.same(host(got[1]), z)
+    L.same(host(got[0]), y, unsure)
+    h, g, u, unsure = L.gated(x, w, w2)
+    got = Z.GatedLinearM31(dev(w), dev(w2))(dev(x), keep=True, x_bits=x_bits)
+    for a, want in zip(got, (h, g, u)):
+        L.same(host(a), want, unsure if want is h else None)
