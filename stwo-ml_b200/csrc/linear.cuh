@@ -65,10 +65,10 @@ struct LinearIO {
     int activation;
     const uint8_t* act_table = nullptr;  // SiLU, GELU: the segment table in device memory
     bool as_reference = false;  // an activation that rounds a negative value to zero gives the word P, not 0
-    uint64_t wait_ns = 2000000000;  // after which a wait inside a kernel gives up: LIN_TIMEOUT
-    // LIN_WITHHOLD_*, none in any call but the self-test's: what block 0 of linear_kernel, or the last
-    // block of cluster 0 of linear_token_kernel, leaves undone so that a wait runs out.
+    // The self-test's alone: LIN_WITHHOLD_*, what block 0 of linear_kernel, or the last block of cluster 0 of
+    // linear_token_kernel, leaves undone so that a wait runs out, and the waits' limit.
     int withhold = 0;
+    uint64_t wait_ns = 0;
 };
 constexpr int LIN_WITHHOLD_DONE = 1;    // the commit of its (first) accumulators: the finishing warps wait
 constexpr int LIN_WITHHOLD_COPY = 2;    // the copies from a weight tile on: the products' issuer waits

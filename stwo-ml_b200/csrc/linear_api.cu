@@ -457,8 +457,8 @@ static int forward(zkml_linear* lin, const zkml_linear_call* c, uint32_t* status
     io.m = (uint32_t)m;
     io.activation = c->activation;
     io.act_table = c->activation == 2 ? lin->act_table[0] : c->activation == 5 ? lin->act_table[1] : nullptr;
-    if (wait_ns) io.wait_ns = wait_ns;
     io.withhold = withhold;
+    io.wait_ns = wait_ns;
     const Choice& p = choose(lin->w, io.m, c->x_bits, ctx->num_sms);
     if ((withhold == LIN_WITHHOLD_TABLE && (p.few || !io.act_table)) || (withhold == LIN_WITHHOLD_DIGITS && !p.few))
         return set_error(ZKML_ERR_INVALID_ARG, "the kernel of this call has no such wait");

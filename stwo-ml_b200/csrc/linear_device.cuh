@@ -231,6 +231,25 @@ __device__ __forceinline__ void finish_tokens(const LinearIO& io, const uint8_t*
     }
 }
 
+// What a block whose waits ran out does before it gives up its tensor memory and ends: it says so, and lets
+// the copies (the last `issued` of a ring of stages, and the one behind bar2 if that is not 0) and products
+// in flight end.  Out of line: no ordinary block comes here.
+static __device__ __noinline__ void report_timeout(uint32_t* status, uint32_t full, uint32_t stages, uint32_t issued,
+                                                   uint32_t bar2, uint64_t wait_ns) {
+    volatile uint32_t never = 0;
+    atomicOr(status, LIN_TIMEOUT);
+    for (uint32_t i = 0; i < min(issued, stages); i++) {  // a barrier may also lack an arrival: then the limit ends it
+        const uint32_t u = issued - 1 - i;
+        mbar_wait(full + 8 * (u % stages), (u / stages) & 1, &never, wait_ns);
+    }
+    if (bar2) mbar_wait(bar2, 0, &never, wait_ns);
+}
+static __device__ __noinline__ void drain_products(uint32_t drained, uint64_t wait_ns) {
+    volatile uint32_t never = 0;
+    tc_commit(drained);
+    mbar_wait(drained, 0, &never, wait_ns);
+}
+
 // Both kernels of a call are programmatic dependents: a block of the product kernel starts, and
 // loads weights, as soon as an SM is free, before the digits are made and before the last blocks
 // of the previous call are done; what depends on earlier work comes after grid_dependency_wait.

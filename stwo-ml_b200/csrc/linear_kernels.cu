@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
     __shared__ uint32_t tmem_base_s, last_s, issued_s;
     __shared__ volatile uint32_t quit_s;
     constexpr int G = GROUP<D>;
+    const uint64_t wait_ns = SELFTEST ? a.io.wait_ns : WAIT_NS;
     const int withhold = SELFTEST && blockIdx.x == 0 ? a.io.withhold : 0;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t n_cols = D * a.tokens, b_bytes = n_cols * LIN_KB, stage_bytes = LIN_TILE_BYTES + b_bytes;
@@ -344,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
                     bulk_load(smem0 + i * stage_bytes + LIN_TILE_BYTES, first_x[i], b_bytes, full + 8 * i);
             uint32_t st = 0, phase = 0;
             while (more && issued >= a.stages && advance()) {
-                if (!mbar_wait(empty + 8 * st, phase, &quit_s, a.io.wait_ns)) break;
+                if (!mbar_wait(empty + 8 * st, phase, &quit_s, wait_ns)) break;
                 mbar_expect_tx(full + 8 * st, stage_bytes);
                 bulk_load(smem0 + st * stage_bytes, wp, LIN_TILE_BYTES, full + 8 * st);
                 bulk_load(smem0 + st * stage_bytes + LIN_TILE_BYTES, xp, b_bytes, full + 8 * st);
@@ -365,11 +366,11 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
             bool ok = true;
             while (ok && sch.next(s)) {
                 const uint32_t buf = seg & 1, use = seg >> 1;
-                ok = mbar_wait(acc_empty + 8 * buf, (use & 1) ^ 1, &quit_s, a.io.wait_ns);
+                ok = mbar_wait(acc_empty + 8 * buf, (use & 1) ^ 1, &quit_s, wait_ns);
                 tc_fence_after();
                 const uint32_t d = tmem + buf * (cols / 2);
                 for (uint32_t u = 0; ok && u < s.len; u++) {
-                    if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s, a.io.wait_ns))) break;
+                    if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s, wait_ns))) break;
                     tc_fence_after();
                     const uint64_t da = tc_desc_k128(smem0 + st * stage_bytes);
                     const uint64_t db = tc_desc_k128(smem0 + st * stage_bytes + LIN_TILE_BYTES);
@@ -390,13 +391,13 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
         sch.init(a);
         Segment s{};
         uint32_t seg = 0;
-        const bool have_table = !bends || mbar_wait(table_full, 0, &quit_s, a.io.wait_ns);
+        const bool have_table = !bends || mbar_wait(table_full, 0, &quit_s, wait_ns);
         const uint8_t* table = smem_raw + (table_at - smem_addr(smem_raw));
         uint32_t* const my_slots = a.slots + (size_t)blockIdx.x * a.slots_per_cta * a.tokens * LIN_ROWS;
         while (sch.next(s)) {
             const uint32_t buf = seg & 1, use = seg >> 1;
             seg++;
-            if (!all_of_epilogue(have_table && mbar_wait(acc_full + 8 * buf, use & 1, &quit_s, a.io.wait_ns))) break;
+            if (!all_of_epilogue(have_table && mbar_wait(acc_full + 8 * buf, use & 1, &quit_s, wait_ns))) break;
             tc_fence_after();
             uint32_t mt, nt;
             tile_at(a, s.tile, mt, nt);
@@ -483,21 +484,9 @@ __global__ void __launch_bounds__(THREADS, 1) linear_kernel(const __grid_constan
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (quit_s) {
-        // some role's wait ran out (all roles are done now): reported, and the copies and products still in
-        // flight end before the tensor memory and the block do
-        volatile uint32_t never = 0;
-        if (threadIdx.x == 0) {
-            atomicOr(a.io.status, LIN_TIMEOUT);
-            for (uint32_t i = 0; i < min(issued_s, a.stages); i++) {
-                const uint32_t u = issued_s - 1 - i;
-                mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never, a.io.wait_ns);
-            }
-            if (bends) mbar_wait(table_full, 0, &never, a.io.wait_ns);
-        } else if (threadIdx.x == 32) {  // the products' issuer
-            tc_commit(drained);
-            mbar_wait(drained, 0, &never, a.io.wait_ns);
-        }
+    if (quit_s) {  // some role's wait ran out (all roles are done now)
+        if (threadIdx.x == 0) report_timeout(a.io.status, full, a.stages, issued_s, bends ? table_full : 0, wait_ns);
+        if (threadIdx.x == 32) drain_products(drained, wait_ns);  // by their issuer
         __syncwarp();
         __syncthreads();
     }

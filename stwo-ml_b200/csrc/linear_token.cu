@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
     constexpr int G = GROUP<D>;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t nt = blockIdx.x / a.parts, rank = blockIdx.x % a.parts;  // cluster dimension: parts
+    const uint64_t wait_ns = SELFTEST ? a.io.wait_ns : WAIT_NS;
     const int withhold = SELFTEST && nt == 0 && rank + 1 == a.parts ? a.io.withhold : 0;
     const uint32_t n_cols = D * a.tokens, stage_bytes = LIN_TILE_BYTES + n_cols * LIN_KB;
     const uint32_t smem0 = (smem_addr(smem_raw) + 1023) & ~1023u;
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             uint32_t st = 0, phase = 1, issued = 0;
             for (uint32_t u = 0; u < units; u++) {
                 if (u == a.stages) grid_dependency_wait();  // so that the waits' limit counts this grid's own time alone
-                if (!(ok = mbar_wait(empty + 8 * st, phase, &quit_s, a.io.wait_ns))) break;
+                if (!(ok = mbar_wait(empty + 8 * st, phase, &quit_s, wait_ns))) break;
                 if (SELFTEST && withhold == LIN_WITHHOLD_COPY && u + 1 == units) break;
                 uint32_t plane, kt;
                 tile_of(u, plane, kt);
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             const uint32_t idesc = tc_idesc_s8(n_cols);
             uint32_t st = 0, phase = 0, kt_done = 0, plane = 0;
             for (uint32_t u = 0; u < units; u++) {
-                if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s, a.io.wait_ns))) break;
+                if (!(ok = mbar_wait(full + 8 * st, phase, &quit_s, wait_ns))) break;
                 tc_fence_after();
                 const uint64_t da = tc_desc_k128(smem0 + st * stage_bytes);
                 const uint64_t db = tc_desc_k128(smem0 + st * stage_bytes + LIN_TILE_BYTES);
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
             if (u_next < units) load(ahead, u_next);  // on its way while this one becomes digits
             const uint32_t st = u % a.stages, tile = smem0 + st * stage_bytes + LIN_TILE_BYTES;
             // the stage's last product is done
-            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ((u / a.stages) & 1) ^ 1, &quit_s, a.io.wait_ns));
+            ok = __all_sync(0xffffffffu, mbar_wait(empty + 8 * st, ((u / a.stages) & 1) ^ 1, &quit_s, wait_ns));
             if (!ok) break;
 #pragma unroll
             for (uint32_t i = 0; i < 2; i++) {
@@ -188,7 +189,7 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
         if (bad) atomicOr(a.io.status, bad);
         // ---- this warp's quarter of the rows (warps 2 to 5): TMEM lanes 32 (warp % 4) and up
         if (maker < 4 && __all_sync(0xffffffffu, ok)) {
-            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, &quit_s, a.io.wait_ns));
+            ok = __all_sync(0xffffffffu, mbar_wait(acc_full, 0, &quit_s, wait_ns));
             tc_fence_after();
             if (ok) {
 #pragma unroll
@@ -266,20 +267,9 @@ __global__ void __launch_bounds__(TOKEN_THREADS, 2) linear_token_kernel(const __
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (quit_s) {
-        // some role's wait ran out (all roles are done now): reported, and the copies and products still in
-        // flight end before the tensor memory and the block do
-        volatile uint32_t never = 0;
-        if (threadIdx.x == 0) {
-            atomicOr(a.io.status, LIN_TIMEOUT);
-            for (uint32_t i = 0; i < min(issued_s, a.stages); i++) {  // a barrier may lack the digits' arrival: then the limit ends it
-                const uint32_t u = issued_s - 1 - i;
-                mbar_wait(full + 8 * (u % a.stages), (u / a.stages) & 1, &never, a.io.wait_ns);
-            }
-        } else if (threadIdx.x == 32) {  // the products' issuer
-            tc_commit(drained);
-            mbar_wait(drained, 0, &never, a.io.wait_ns);
-        }
+    if (quit_s) {  // some role's wait ran out (all roles are done now)
+        if (threadIdx.x == 0) report_timeout(a.io.status, full, a.stages, issued_s, 0, wait_ns);
+        if (threadIdx.x == 32) drain_products(drained, wait_ns);  // by their issuer
         __syncwarp();
         __syncthreads();
     }

@@ -46,6 +46,8 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+constexpr uint64_t WAIT_NS = 2000000000;  // a wait's limit, in every kernel but a self-test's
+
 // bytes (a multiple of 16) from global to this block's shared memory, both 16-byte aligned.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
