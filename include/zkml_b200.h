@@ -398,9 +398,9 @@ int zkml_matmul_m31(zkml_ctx *ctx, const uint32_t *a, size_t m, size_t k, const 
  * y = f(x W + b) + r and the gated block's h = f(x Wg + bg) * (x Wu + bu), mod p: what a
  * Linear layer with its activation and residual, and a gated feed-forward block, compute
  * before they are proved.  Exact for every M31 input.  A zkml_linear holds the weights in the
- * layout the kernels read; it belongs to the context it was made with, is destroyed before
- * it, and is not changed by calls, so calls on several streams (each with a workspace of its
- * own) may use it at once. */
+ * layout the kernels read; it belongs to the context it was made with and is destroyed before
+ * it.  Calls change nothing of it but the record of what they met, so calls of several threads and
+ * streams (each with a workspace of its own) may use it at once. */
 typedef struct zkml_linear zkml_linear;
 
 /* Lay out W (k x n; element (i, j) at w[i * row_stride + j * col_stride], strides in words, so
@@ -424,7 +424,7 @@ int zkml_linear_destroy(zkml_linear *lin);
  * out may be the residual itself (same pointer and stride). */
 typedef struct {
     const uint32_t *x; /* m x k activations */
-    size_t m, ldx;
+    size_t m, ldx;     /* m at least 1 */
     int x_bits;     /* width the activations are quantised to: 8 ([-128, 127]), 16, or 31 (any element) */
     int activation; /* f: 0 none, or a type tag (1 ReLU, 2 GELU, 3 Sigmoid, 4 Softmax-exp, 5 SiLU), applied
                        to full M31 values as in zkml_prove_gkr_chain's forward pass; canonical result */

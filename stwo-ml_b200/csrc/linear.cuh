@@ -110,8 +110,8 @@ cudaError_t launch_linear(const PackedWeights& w, const LinearPlan& p, const Lin
 // One product with weights that are used once (the chain prover's forward pass): lays w (k x n,
 // row major, host or device memory) out in the context's scratch and runs the call on its stream.
 // x, residual, pre and out are dense device matrices; pre may be NULL.  ZKML_ERR_OOM leaves
-// nothing done and no scratch of its own held.  A run of calls is opened by _begin and closed by _end, which waits for the stream
-// and reports what the calls met.
+// nothing done and no scratch held.  A run of calls is opened by _begin and closed by _end, which waits
+// for the stream and reports what the calls met.  The weights' layout is in op.bmle until then.
 int linear_once_begin(::zkml_ctx* ctx);
 int linear_once_end(::zkml_ctx* ctx);
 int linear_once(::zkml_ctx* ctx, const uint32_t* x, size_t m, size_t k, const uint32_t* w, size_t n, int activation,

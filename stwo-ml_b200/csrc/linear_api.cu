@@ -429,17 +429,21 @@ static int forward(zkml_linear* lin, const zkml_linear_call* c, uint32_t* status
                               reinterpret_cast<uintptr_t>(c->up);
         if (all & 3) return set_error(ZKML_ERR_INVALID_ARG, "an argument is not aligned to words");
     } else if ((rc = want_device_words(ctx, c->x, "x")) || (rc = want_device_words(ctx, c->out, "out")) ||
-        (need && (rc = want_device_words(ctx, c->workspace, "workspace"))) ||
-        (c->residual && (rc = want_device_words(ctx, c->residual, "residual"))) ||
-        (c->pre && (rc = want_device_words(ctx, c->pre, "pre"))) ||
-        (c->up && (rc = want_device_words(ctx, c->up, "up"))))
+               (need && (rc = want_device_words(ctx, c->workspace, "workspace"))) ||
+               (c->residual && (rc = want_device_words(ctx, c->residual, "residual"))) ||
+               (c->pre && (rc = want_device_words(ctx, c->pre, "pre"))) ||
+               (c->up && (rc = want_device_words(ctx, c->up, "up"))))
         return rc;
     const Block x{c->x, m, k, c->ldx}, res{c->residual, m, n, c->ld_residual}, out{c->out, m, n, c->ld_out};
     const Block pre{c->pre, m, n, c->ld_pre}, up{c->up, m, n, c->ld_up};
     const Block wsp{need ? static_cast<const uint32_t*>(c->workspace) : nullptr, 1, need / 4, 0};
     const bool in_place = c->residual == c->out && c->ld_residual == c->ld_out;
-    if (share(wsp, x) || share(wsp, out) || share(wsp, pre) || share(wsp, up) || share(wsp, res) || share(out, x) || share(pre, x) || share(up, x) || share(out, pre) || share(out, up) || share(pre, up) ||
-        (!in_place && share(out, res)) || share(pre, res))
+    const bool with_inputs = share(out, x) || share(pre, x) || share(up, x) || share(pre, res) ||
+                             (!in_place && share(out, res));
+    const bool with_outputs = share(out, pre) || share(out, up) || share(pre, up);
+    const bool with_workspace =
+        share(wsp, x) || share(wsp, res) || share(wsp, out) || share(wsp, pre) || share(wsp, up);
+    if (with_inputs || with_outputs || with_workspace)
         return set_error(ZKML_ERR_INVALID_ARG, "an output overlaps another argument");
     cudaStream_t s = c->stream ? static_cast<cudaStream_t>(c->stream) : ctx->stream;
     LinearIO io{};

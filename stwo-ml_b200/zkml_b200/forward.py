@@ -269,7 +269,7 @@ class LinearM31(_Weights):
 
     def __call__(self, x, activation=None, residual=None, out=None, pre=None, keep: bool = False, x_bits: int = 31,
                  check: bool = True):
-        """x: (..., k); returns y (..., n), or (y, x W + b) with keep (or a tensor for pre).
+        """x: (..., k), of at least one row; returns y (..., n), or (y, x W + b) with keep (or a tensor for pre).
 
         activation: None, "relu", "gelu", "sigmoid", "softmax", "silu" or a type tag; residual: as y, or
         one row of n words for all; out / pre: int32 tensors to write, of any row stride (out may be the
