@@ -421,3 +421,88 @@ def test_wide_weights_over_a_cluster(k, w_bits, m, x_bits):
     got = Z.GatedLinearM31(dev(w), dev(w2))(dev(x), keep=True, x_bits=x_bits)
     for a, want in zip(got, (h, g, u)):
         L.same(host(a), want, unsure if want is h else None)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("m", [1, 40])
+def test_inputs_written_late_on_another_stream(m, captured):
+    """A call behind another call of its stream and an event of a second stream: it starts early for the first,
+    and still waits for the second."""
+    k, n = 600, 300
+    x, w = ints((m, k), 31, 1), ints((k, n), 8, 2)
+    lin, other, want = Z.LinearM31(dev(w)), Z.LinearM31(dev(w)), L.product(x, w)
+    source, tx = dev(x), torch.zeros(m, k, dtype=torch.int32, device="cuda")
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def step():
+        s1.wait_stream(s2)
+        with torch.cuda.stream(s1):
+            torch.cuda._sleep(2_000_000)
+            tx.copy_(source)
+        with torch.cuda.stream(s2):
+            other(source, check=False)
+            s2.wait_stream(s1)
+            y = lin(tx, check=False)
+            z = other(tx, residual=y, check=False)
+            tx.zero_()  # the calls have read it by then
+        return y, z
+
+    torch.cuda.synchronize()
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s2):
+            y, z = step()
+    for _ in range(4):
+        if captured:
+            g.replay()
+        else:
+            y, z = step()
+        torch.cuda.synchronize()
+        L.same(host(y), want)
+        L.same(host(z), 2 * want % P)
+    lin.check()
+    other.check()
+
+
+@pytest.mark.parametrize("m", [9, 1])
+def test_rows_further_apart_than_32_bits(m):
+    """x, residual, input of the activation and result as column ranges of one buffer whose rows are 2^29 words
+    apart: the ninth row begins 2^32 words in."""
+    k, n, ld = 300, 130, 1 << 29
+    x, w, r = ints((10, k), 8, 1), ints((k, n), 8, 2), ints((10, n), 31, 3)
+    buf = torch.empty(9 * ld + 4096, dtype=torch.int32, device="cuda")
+    first = 10 - m  # one token: the last row alone, at its own offset
+    rows = torch.as_strided(buf, (m, 4096), (ld, 1), first * ld if m == 1 else 0)
+    rows.fill_(MARK)
+    at = {"x": (7, k), "r": (400, n), "z": (700, n), "y": (1001, n)}
+    part = {name: rows[:, a:a + width] for name, (a, width) in at.items()}
+    part["x"].copy_(dev(x[first:]))
+    part["r"].copy_(dev(r[first:]))
+    y, z, unsure = L.linear(x[first:], w, None, 5, r[first:])
+    Z.LinearM31(dev(w))(part["x"], activation="silu", residual=part["r"], out=part["y"], pre=part["z"], x_bits=8)
+    L.same(host(part["y"].contiguous()), y, unsure)
+    L.same(host(part["z"].contiguous()), z)
+    rest = torch.ones(m, 4096, dtype=torch.bool, device="cuda")
+    for a, width in at.values():
+        rest[:, a:a + width] = False
+    assert (rows[rest] == MARK).all()
+
+
+@pytest.mark.parametrize("gap", [0, 3])
+@pytest.mark.parametrize("m", [1, 7, 24, 200])
+def test_calls_that_read_what_the_call_before_wrote_beside_its_input(m, gap):
+    """Two column ranges of one buffer in turn, input and result of one call sharing sectors: what is kept of a
+    range from an earlier read never stands for what has been written since."""
+    d = 137
+    w, x = ints((d, d), 31, 1), ints((m, d), 31, 2)
+    lin = Z.LinearM31(dev(w))
+    buf = torch.zeros(m, 2 * d + gap + 5, dtype=torch.int32, device="cuda")
+    parts = [buf[:, 1:1 + d], buf[:, 1 + d + gap:1 + 2 * d + gap]]
+    parts[0].copy_(dev(x))
+    torch.cuda._sleep(5_000_000)  # the calls queue up and start early
+    want = x
+    for i in range(40):
+        lin(parts[i % 2], out=parts[1 - i % 2], check=False)
+        want = L.product(want, w)
+    L.same(host(parts[0].contiguous()), want)
+    lin.check()
